@@ -548,6 +548,111 @@ int ttl_qkv_rope_store(ttl_ctx *ctx, const float *qkv_dev, uint32_t tokens, uint
  * 545-551). */
 int ttl_add(ttl_ctx *ctx, const float *a_dev, const float *b_dev, size_t n, float *out_dev);
 
+/* ---- paged 4-bit KV cache: several sequences, long contexts ------------------------- *
+ * The keys and values of many sequences in one pool of pages, as MXFP4 blocks: the store of
+ * new tokens, attention of one token per sequence and of runs of prompt tokens, and the
+ * values back in f32.  The counterparts over one sequence's dense f32 cache are
+ * ttl_qkv_rope_store, ttl_attention_decode and ttl_attention_prefill; a cached position takes
+ * kv_heads x (head_dim + head_dim / 16) bytes, 544 at gpt-oss's shape against 4096 in f32.
+ * No reference counterpart: the reference serves one sequence from an f32 cache
+ * (model.cpp:171-172, 247-253).
+ *
+ * pool is uint8 [pages][kv_heads][record] (ttl_kv4_pool_bytes, 16-byte aligned), a record being
+ *   K codes [page_positions][head_dim / 2], V codes [page_positions][head_dim / 2],
+ *   K scales [page_positions][head_dim / 32], V scales [page_positions][head_dim / 32];
+ * code byte j of a position holds dims 2j (low nibble) and 2j + 1.  32 dims of one head and
+ * position form a block: E8M0 byte e + 127 for the smallest e in -126..125 with every
+ * magnitude below 7 x 2^e, so that the largest rounds to 6 x 2^e at most, and E2M1 codes of
+ * x / 2^e rounded to nearest, ties to the even code (6 x 2^125 where x is larger).  Byte 0
+ * marks a block whose codes are all zero; byte 255 one with a value that is no finite f32,
+ * which reads as NaN.
+ *
+ * A pool's contents need no initialisation: only positions below a sequence's length are
+ * ever used. */
+typedef struct {
+    uint32_t kv_heads;        /* 1..256                                                 */
+    uint32_t head_dim;        /* 64 or 128                                              */
+    uint32_t page_positions;  /* 16, 32, 64, 128 or 256                                 */
+    uint32_t pages;           /* pages of the pool, 1..2^31 - 1                         */
+    uint8_t *pool;            /* device memory                                          */
+} ttl_kv4_cache;
+
+/* The sequences of a call and the rows (tokens) of its arrays.  Sequence s holds lengths[s]
+ * positions, the call's own tokens included; its rows are starts[s] .. starts[s + 1] - 1, at
+ * its last positions in order.  starts NULL: one row per sequence (tokens == sequences).
+ * starts[0] = 0 and starts never decreases; rows from starts[sequences] on are padding, and
+ * what belongs to them is neither read nor written.  Position p of sequence s lies in page
+ * page_table[s][p / page_positions] (entries that hold no used position may be anything).
+ * The arrays are in device memory, so one captured call serves every step; what they hold
+ * is bounds-checked by the kernels: a row before position 0 (a sequence of length 0: an idle
+ * slot of a batch, or more rows than positions) gets zeros, and a row whose sequence is longer
+ * than max_length, or needs a page outside the pool, gets NaN. */
+typedef struct {
+    uint32_t sequences;         /* 0..2^20                                              */
+    uint32_t tokens;            /* rows, 0..2^24                                        */
+    uint32_t table_stride;      /* page-table entries per sequence                      */
+    uint32_t max_length;        /* at least every length; at most table_stride x page_positions and 2^30 */
+    const int32_t *page_table;  /* int32 [sequences][table_stride]                      */
+    const int32_t *lengths;     /* int32 [sequences]                                    */
+    const int32_t *starts;      /* int32 [sequences + 1], or NULL                       */
+} ttl_kv4_batch;
+
+/* The attention of a call: query head h reads key/value head h / (heads / kv_heads); position
+ * p sees positions max(0, p + 1 - window) .. p. */
+typedef struct {
+    uint32_t heads;      /* a multiple of kv_heads, at most 64 per key/value head       */
+    uint32_t window;     /* positions a token sees, its own included; 0: all            */
+    float scale;         /* of the scores, 1/sqrt(head_dim) as a rule; finite           */
+    int dtype;           /* of q and out: TTL_DTYPE_F32 or TTL_DTYPE_BF16               */
+    const float *sinks;  /* f32 [heads], or NULL: no sinks                              */
+} ttl_kv4_attention;
+
+/* Bytes of a pool; 0 for a shape the kernels do not support. */
+size_t ttl_kv4_pool_bytes(const ttl_kv4_cache *cache);
+
+/* ttl_qkv_rope_store for a batch over the paged cache: qkv_dev [tokens][(heads + 2 kv_heads)
+ * head_dim] of x_dtype (TTL_DTYPE_F32 or TTL_DTYPE_BF16) holds the projections without their
+ * bias, in the order q | k | v, or, with qkv_order TTL_QKV_TILED, in that of
+ * ttl_qkv_row_source (64 query and 8 key/value heads of 64).  bias_dev f32, in q | k | v order,
+ * may be NULL.  Pairs (d, d + head_dim / 2) of q and k are turned by rope_dev f32
+ * [rope_positions][head_dim / 2][2] = (cos, sin) times any factor, as ttl_attn_qkv takes it.
+ * q_dev [tokens][heads][head_dim] of q_dtype receives the queries; k and v go to the cache.
+ * Bias and rotation are computed in 64 bits, so q is rounded once and a code is the nearest
+ * one of the exact value.  A row at a position from rope_positions on counts as one of a too
+ * long sequence: nothing is stored for such rows.  No two rows may share a position of a
+ * page.  qkv, bias, rope and q 16-byte aligned. */
+#define TTL_QKV_PLAIN 0
+#define TTL_QKV_TILED 1
+int ttl_qkv_rope_store_kv4(ttl_ctx *ctx, const ttl_kv4_cache *cache, const ttl_kv4_batch *batch, uint32_t heads,
+                           const void *qkv_dev, int x_dtype, int qkv_order, const float *bias_dev,
+                           const float *rope_dev, uint32_t rope_positions, void *q_dev, int q_dtype);
+
+/* k and v of the batch's rows as the cache holds them: f32 [tokens][kv_heads][head_dim] each
+ * (either may be NULL), 16-byte aligned.  With starts at every length's running sum it returns
+ * whole sequences, for instance to continue one in a dense f32 cache. */
+int ttl_kv4_dequantize(ttl_ctx *ctx, const ttl_kv4_cache *cache, const ttl_kv4_batch *batch, float *k_dev,
+                       float *v_dev);
+
+/* Device memory that a call of the attention below needs (0: none). */
+size_t ttl_attention_kv4_workspace_bytes(const ttl_kv4_cache *cache, const ttl_kv4_batch *batch,
+                                         const ttl_kv4_attention *attention);
+/* out = softmax(scale q k, sink) v of one token per sequence (batch->starts NULL) at its last
+ * position, the sink in the maximum and the denominator only (model.cpp:270-281): q_dev and
+ * out_dev [sequences][heads][head_dim] of attention->dtype, 16-byte aligned.  A query with a
+ * value that is not finite gives NaN, as does one that sees a NaN block; masked positions
+ * have no influence whatever they hold.  Products, sums and the softmax are f32.
+ * workspace_dev is caller-owned, 256-byte aligned, of the size above; calls sharing one must
+ * not overlap. */
+int ttl_attention_decode_kv4(ttl_ctx *ctx, const ttl_kv4_cache *cache, const ttl_kv4_batch *batch,
+                             const ttl_kv4_attention *attention, const void *q_dev, void *out_dev,
+                             void *workspace_dev, size_t workspace_bytes);
+/* The same for runs of tokens (batch->starts given), prompt passes of several sequences in one
+ * call: q_dev and out_dev [tokens][heads][head_dim].  The cache must hold the rows' own keys
+ * and values already. */
+int ttl_attention_prefill_kv4(ttl_ctx *ctx, const ttl_kv4_cache *cache, const ttl_kv4_batch *batch,
+                              const ttl_kv4_attention *attention, const void *q_dev, void *out_dev,
+                              void *workspace_dev, size_t workspace_bytes);
+
 /* ---- embedding, unembedding, greedy ------------------------------------------------ */
 
 /* load_token_embedding_q8_0 (tensor.cpp:171-184) for the token in token_dev; table_dev

@@ -21,6 +21,7 @@ TTL_DTYPE_F32_AS_MXFP8 = 2
 TTL_DTYPE_BF16_AS_MXFP8 = 3
 TTL_PREFILL_PLAN, TTL_PREFILL_GATHER, TTL_PREFILL_GATEUP, TTL_PREFILL_DOWN, TTL_PREFILL_COMBINE = 1, 2, 4, 8, 16
 TTL_PREFILL_ALL = 31
+TTL_QKV_PLAIN, TTL_QKV_TILED = 0, 1
 
 
 class TtlError(RuntimeError):
@@ -70,6 +71,56 @@ def stage_input(base, add=None, add_weights=None, add_count=0, norm=None, eps=1e
     s.epsilon = eps
     s.sum_out = sum_out.ptr if sum_out else None
     return s
+
+
+class Kv4CacheDesc(C.Structure):
+    """Mirror of ttl_kv4_cache."""
+    _fields_ = [("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("page_positions", C.c_uint32),
+                ("pages", C.c_uint32), ("pool", C.c_void_p)]
+
+
+class Kv4BatchDesc(C.Structure):
+    """Mirror of ttl_kv4_batch."""
+    _fields_ = [("sequences", C.c_uint32), ("tokens", C.c_uint32), ("table_stride", C.c_uint32),
+                ("max_length", C.c_uint32), ("page_table", C.c_void_p), ("lengths", C.c_void_p),
+                ("starts", C.c_void_p)]
+
+
+class Kv4AttentionDesc(C.Structure):
+    """Mirror of ttl_kv4_attention."""
+    _fields_ = [("heads", C.c_uint32), ("window", C.c_uint32), ("scale", C.c_float), ("dtype", C.c_int),
+                ("sinks", C.c_void_p)]
+
+
+def _address(x):
+    """The device address of a Buffer, or an address as it is (an int, a c_void_p, None)."""
+    return x.ptr if isinstance(x, Buffer) else x
+
+
+def kv4_cache(pool, pages, kv_heads=8, head_dim=64, page_positions=64):
+    """A paged 4-bit K/V cache over `pool`, device memory of kv4_pool_bytes()."""
+    return Kv4CacheDesc(kv_heads, head_dim, page_positions, pages, _address(pool))
+
+
+def kv4_pool_bytes(pages, kv_heads=8, head_dim=64, page_positions=64):
+    n = load_library().ttl_kv4_pool_bytes(C.byref(kv4_cache(None, pages, kv_heads, head_dim, page_positions)))
+    if n == 0:
+        _check(-2, "ttl_kv4_pool_bytes")
+    return n
+
+
+def kv4_batch(sequences, tokens, page_table, table_stride, lengths, starts=None, max_length=None, page_positions=64):
+    """The sequences of a call: device arrays of page_table int32 [sequences][table_stride],
+    lengths int32 [sequences] and starts int32 [sequences + 1] (None: one token each).
+    max_length (at least every length): by default what the page table can hold."""
+    if max_length is None:
+        max_length = table_stride * page_positions
+    return Kv4BatchDesc(sequences, tokens, table_stride, max_length, _address(page_table), _address(lengths),
+                        _address(starts))
+
+
+def kv4_attention(heads, dtype=TTL_DTYPE_F32, window=0, scale=0.125, sinks=None):
+    return Kv4AttentionDesc(heads, window, scale, dtype, _address(sinks))
 
 
 _lib = None
@@ -406,6 +457,16 @@ def load_library():
         "ttl_matmul_q8_0_workspace_bytes": (sz, [u32, u32]),
         "ttl_matmul_q8_0": (i32, [vp, vp, vp, vp, u32, vp, vp, vp, sz]),
         "ttl_matmul_q8_0_shifted": (i32, [vp, vp, vp, vp, vp, u32, vp, vp, vp, sz]),
+        "ttl_kv4_pool_bytes": (sz, [C.POINTER(Kv4CacheDesc)]),
+        "ttl_qkv_rope_store_kv4": (i32, [vp, C.POINTER(Kv4CacheDesc), C.POINTER(Kv4BatchDesc), u32, vp, i32, i32, vp,
+                                         vp, u32, vp, i32]),
+        "ttl_kv4_dequantize": (i32, [vp, C.POINTER(Kv4CacheDesc), C.POINTER(Kv4BatchDesc), vp, vp]),
+        "ttl_attention_kv4_workspace_bytes": (sz, [C.POINTER(Kv4CacheDesc), C.POINTER(Kv4BatchDesc),
+                                                   C.POINTER(Kv4AttentionDesc)]),
+        "ttl_attention_decode_kv4": (i32, [vp, C.POINTER(Kv4CacheDesc), C.POINTER(Kv4BatchDesc),
+                                           C.POINTER(Kv4AttentionDesc), vp, vp, vp, sz]),
+        "ttl_attention_prefill_kv4": (i32, [vp, C.POINTER(Kv4CacheDesc), C.POINTER(Kv4BatchDesc),
+                                            C.POINTER(Kv4AttentionDesc), vp, vp, vp, sz]),
         "ttl_capture_begin": (i32, [vp]),
         "ttl_capture_end": (i32, [vp, C.POINTER(vp)]),
         "ttl_graph_launch": (i32, [vp, vp]),
@@ -799,6 +860,34 @@ class Device:
     def attention_prefill(self, q, kc, vc, sinks, first, tokens, capacity, layer_index, out):
         _check(self.lib.ttl_attention_prefill(self.ctx, q.ptr, kc.ptr, vc.ptr, sinks.ptr, first, tokens, capacity,
                                               layer_index, out.ptr), "ttl_attention_prefill")
+
+    # ---- paged 4-bit K/V cache (buffers, or device addresses as integers) ----
+    def qkv_rope_store_kv4(self, cache, batch, heads, qkv, x_dtype, bias, rope, rope_positions, q, q_dtype,
+                           tiled=False):
+        """Bias, rotation and store of the batch's new tokens; q receives the queries."""
+        _check(self.lib.ttl_qkv_rope_store_kv4(self.ctx, C.byref(cache), C.byref(batch), heads, _address(qkv), x_dtype,
+                                               TTL_QKV_TILED if tiled else TTL_QKV_PLAIN, _address(bias),
+                                               _address(rope), rope_positions, _address(q), q_dtype),
+               "ttl_qkv_rope_store_kv4")
+
+    def kv4_dequantize(self, cache, batch, k, v):
+        _check(self.lib.ttl_kv4_dequantize(self.ctx, C.byref(cache), C.byref(batch), _address(k), _address(v)),
+               "ttl_kv4_dequantize")
+
+    def attention_kv4_workspace_bytes(self, cache, batch, attention):
+        return self.lib.ttl_attention_kv4_workspace_bytes(C.byref(cache), C.byref(batch), C.byref(attention))
+
+    def attention_decode_kv4(self, cache, batch, attention, q, out, workspace=None, workspace_bytes=0):
+        """One token per sequence; workspace: device memory of attention_kv4_workspace_bytes()."""
+        _check(self.lib.ttl_attention_decode_kv4(self.ctx, C.byref(cache), C.byref(batch), C.byref(attention),
+                                                 _address(q), _address(out), _address(workspace), workspace_bytes),
+               "ttl_attention_decode_kv4")
+
+    def attention_prefill_kv4(self, cache, batch, attention, q, out, workspace=None, workspace_bytes=0):
+        """Runs of tokens (the batch has starts)."""
+        _check(self.lib.ttl_attention_prefill_kv4(self.ctx, C.byref(cache), C.byref(batch), C.byref(attention),
+                                                  _address(q), _address(out), _address(workspace), workspace_bytes),
+               "ttl_attention_prefill_kv4")
 
     def embedding_q8_0(self, table, vocab, token, out):
         _check(self.lib.ttl_embedding_q8_0(self.ctx, table.ptr, vocab, token.ptr, out.ptr), "ttl_embedding_q8_0")
