@@ -109,7 +109,8 @@ def rotate(x, bias, rope, positions, heads, kv_heads, hd):
 def attention(q, k, v, positions, first, window, scale, sinks):
     """q f64 [rows][heads][hd] at `positions` over k, v f64 [n][kv_heads][hd] of positions
     first ..; returns the outputs and, per output, sum p |v| / den (what rounding errors of
-    the weights scale with) and per row and head the largest sum |q| |k| scale."""
+    the weights scale with), per row and head the largest sum |q| |k| scale, and per output
+    the sum of the |v| that it sees."""
     rows, heads, hd = q.shape
     group = heads // k.shape[1]
     at = first + np.arange(len(k))[None]
@@ -119,6 +120,7 @@ def attention(q, k, v, positions, first, window, scale, sinks):
     out = np.zeros(q.shape)
     mag = np.zeros(q.shape)
     smax = np.zeros((rows, heads))
+    vsum = np.zeros(q.shape)
     for h in range(heads):
         g = h // group
         with np.errstate(invalid="ignore"):
@@ -135,7 +137,8 @@ def attention(q, k, v, positions, first, window, scale, sinks):
                 w, vv = p[r][seen[r]], v[:, g][seen[r]]
                 out[r, h] = w @ vv / den[r]
                 mag[r, h] = w @ np.abs(vv) / den[r]
-    return out, mag, smax
+                vsum[r, h] = np.abs(vv).sum(0)
+    return out, mag, smax, vsum
 
 
 def bf16_round(x):
@@ -149,17 +152,21 @@ def from_bf16(bits):
     return (bits.astype(np.uint32) << 16).view(np.float32)
 
 
-def allowance(ref, mag, smax, n, hd, bf16, vmax):
+def allowance(ref, mag, smax, vsum, n, hd, bf16):
     """How far an output may be from 64 bits.  Scores: hd products summed in f32 in any
     order are off by at most hd 2^-24 of their sum of magnitudes, and the units of log 2 and
     the exponential's own error add 8 roundings of a value of that size; a weight moves by
     twice that (its own and the maximum's).  Weights' and outputs' sums of n terms: n 2^-24
     each, relative to the sum of magnitudes; 32 more roundings for the rest (rescaling, joins,
     the sink, the division).  A bf16 output: the weights in f16 (2^-11) and the output's own
-    rounding (2^-8).  A weight below f32's smallest normal value may be lost, and so may
-    the bits of an output below it."""
+    rounding (2^-8).
+    Small weights: they are held times 2^15, the largest of a running maximum as 2^15, in f16,
+    whose smallest step is 2^-24.  What the last f16 plane rounds off is at most half of it,
+    2^-25 / 2^15 = 2^-40 of that largest weight, which is at most 1 of the final sum: 2^-40 |v|
+    for each position seen.  (It shows where the large weights meet a v of exactly zero, as one
+    in eight E2M1 codes is.)  Below f32's smallest normal value bits of an output may be lost."""
     u = 2.0 ** -24
-    floor = 2.0 ** -120 * vmax + 2.0 ** -133
+    floor = 2.0 ** -40 * vsum + 2.0 ** -133
     rel = 2.0 * (hd + 8) * u * smax[..., None] + (2 * n + 32) * u
     if bf16:
         return mag * (rel + 2.0 ** -11) * 1.01 + 2.0 ** -8 * np.abs(ref) * 1.01 + floor

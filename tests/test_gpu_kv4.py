@@ -263,8 +263,8 @@ def check_attention(got, q, pool, table, lengths, news, heads, dtype, window, sc
         pos = np.arange(first, n)
         k, v = pool.get(table[s], pos)
         at = np.arange(n - m, n)
-        ref, mag, smax = R.attention(q[row:row + m], k, v, at, first, window, scale, sinks)
-        tol = R.allowance(ref, mag, smax, len(pos), pool.hd, dtype == BF16, np.abs(v).max())
+        ref, mag, smax, vsum = R.attention(q[row:row + m], k, v, at, first, window, scale, sinks)
+        tol = R.allowance(ref, mag, smax, vsum, len(pos), pool.hd, dtype == BF16)
         off = np.abs(got[row:row + m] - ref)
         assert np.isfinite(got[row:row + m]).all(), (s, n, m)
         assert (off <= tol).all(), (s, n, m, float((off / np.maximum(tol, 1e-300)).max()))
