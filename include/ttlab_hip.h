@@ -563,9 +563,9 @@ int ttl_add(ttl_ctx *ctx, const float *a_dev, const float *b_dev, size_t n, floa
  * code byte j of a position holds dims 2j (low nibble) and 2j + 1.  32 dims of one head and
  * position form a block: E8M0 byte e + 127 for the smallest e in -126..125 with every
  * magnitude below 7 x 2^e, so that the largest rounds to 6 x 2^e at most, and E2M1 codes of
- * x / 2^e rounded to nearest, ties to the even code (6 x 2^125 where x is larger).  Byte 0
- * marks a block whose codes are all zero; byte 255 one with a value that is no finite f32,
- * which reads as NaN.
+ * x / 2^e rounded to nearest, ties to the even code (6 x 2^125 where x is larger).  A block
+ * whose codes are all zero takes byte 127; byte 255 marks one with a value that is no finite
+ * f32, which reads as NaN.
  *
  * A pool's contents need no initialisation: only positions below a sequence's length are
  * ever used. */

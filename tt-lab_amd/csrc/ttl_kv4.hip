@@ -140,7 +140,7 @@ __device__ inline uint32_t quantise(const double (&x)[4], uint32_t &codes) {
     for (int d = 1; d < 8; d <<= 1) {
         any |= __shfl_xor(any, d);
     }
-    return e == kNone ? 255u : (any ? uint32_t(e + 127) : 0u);
+    return e == kNone ? 255u : (any ? uint32_t(e + 127) : 127u);
 }
 
 // Bias, rotation and store of new tokens.  HD / 8 lanes take one head of one token: lane j

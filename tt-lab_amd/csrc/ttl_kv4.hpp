@@ -102,8 +102,7 @@ __device__ inline uint8_t *record_of(const Cache &c, uint32_t page, uint32_t kv_
 }
 
 // An E8M0 byte as the scale operand of the conversions: 2^(byte - 127); byte 255 is an
-// infinity there and converts every code to NaN; byte 0 (all codes zero) is taken as
-// 2^-127, and gives zeros.
+// infinity there and converts every code to NaN.
 __device__ inline float scale_of(uint32_t byte) {
     return __uint_as_float(byte << 23);
 }

@@ -47,6 +47,7 @@ typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 constexpr uint32_t kChunk = 64, kTiles = kChunk / 16;
 constexpr uint32_t kWaves = 4, kThreads = kWaves * 64;
 constexpr float kLog2e = 0x1.715476p+0f, kLog2eLo = 0x1.4ae0cp-26f;  // log2 e = their sum
+constexpr uint32_t kF16First = 104, kF16Last = 140;                  // scale bytes of V on the f16 path
 constexpr float kWeightShift = 15.0f;                               // weights are held times 2^15
 
 struct Params {
@@ -158,42 +159,90 @@ __device__ __attribute__((always_inline)) inline void load_words(const uint8_t *
     }
 }
 
-// The pages of a chunk's tiles; tiles without a position of lo..hi take the nearest that has.
-struct Pages {
-    uint32_t page[kTiles];
+// Where a chunk's tiles lie: the record of each tile's page and its first slot there.  Tiles
+// without a position of lo..hi take the nearest that has.  Pages of 64 positions and more hold
+// a chunk whole (TP = 1 look-up); smaller ones TP = 4 tiles apart.
+template <int TP>
+struct Places {
+    uint32_t page[TP];
 };
-__device__ __attribute__((always_inline)) inline Pages pages_of(const Cache &c, const int32_t *table, uint32_t chunk,
-                                                                uint32_t lo, uint32_t hi) {
-    Pages p;
+template <int TP>
+__device__ __attribute__((always_inline)) inline Places<TP> places_of(const Cache &c, const int32_t *table,
+                                                                      uint32_t chunk, uint32_t lo, uint32_t hi) {
+    Places<TP> p;
 #pragma unroll
-    for (uint32_t i = 0; i < kTiles; ++i) {
-        const uint32_t tile = min(max(chunk * kTiles + i, lo / 16), hi / 16);
+    for (uint32_t i = 0; i < TP; ++i) {
+        const uint32_t tile = TP == 1 ? chunk * kTiles : min(max(chunk * kTiles + i, lo / 16), hi / 16);
         p.page[i] = uint32_t(table[tile >> (c.page_shift - 4)]);
     }
     return p;
 }
 
+// A lane's offsets in a record's tile.
 template <int HD>
-__device__ __attribute__((always_inline)) inline void load_chunk(const Cache &c, uint32_t kv_head, const Pages &pages,
-                                                                 uint32_t chunk, uint32_t lo, uint32_t hi, uint32_t n,
-                                                                 uint32_t g, Codes<HD> &k, Codes<HD> &v) {
+struct LaneOffsets {
+    uint32_t code, scale;
+    __device__ LaneOffsets(uint32_t n, uint32_t g)
+        : code(n * Layout<HD>::code_bytes + g * (HD / 8)), scale(n * Layout<HD>::scale_bytes + g * (HD / 4) / 32) {}
+};
+
+template <int HD, int TP>
+__device__ __attribute__((always_inline)) inline void load_chunk(const Cache &c, uint32_t kv_head,
+                                                                 const Places<TP> &places, uint32_t chunk, uint32_t lo,
+                                                                 uint32_t hi, const LaneOffsets<HD> &at, Codes<HD> &k,
+                                                                 Codes<HD> &v) {
     using L = Layout<HD>;
+    const uint32_t mask = (1u << c.page_shift) - 1;
+    const uint8_t *kp = nullptr, *vp = nullptr, *ks = nullptr, *vs = nullptr;  // uniform
 #pragma unroll
     for (uint32_t i = 0; i < kTiles; ++i) {
-        const uint32_t tile = min(max(chunk * kTiles + i, lo / 16), hi / 16);
-        const bool in_pool = pages.page[i] < c.pages;
-        const uint32_t slot = (tile * 16) & ((1u << c.page_shift) - 1);
-        const uint8_t *rec = kv4::record_of(c, in_pool ? pages.page[i] : 0u, kv_head);
-        const uint32_t code = n * L::code_bytes + g * (HD / 8), scale = n * L::scale_bytes + g * (HD / 4) / 32;
-        load_words<HD>(rec + L::k_codes(slot) + code, k.w[i]);
-        load_words<HD>(rec + L::v_codes(c.page_shift, slot) + code, v.w[i]);
-        k.scale[i] = rec[L::k_scales(c.page_shift, slot) + scale];
-        v.scale[i] = rec[L::v_scales(c.page_shift, slot) + scale];
-        if (!in_pool) {  // a page that is not there reads as NaN keys
+        if (TP != 1 || i == 0) {
+            const uint32_t tile = TP == 1 ? chunk * kTiles : min(max(chunk * kTiles + i, lo / 16), hi / 16);
+            const uint32_t page = places.page[i], slot = (tile * 16) & mask;
+            const uint8_t *rec = kv4::record_of(c, page < c.pages ? page : 0u, kv_head);
+            kp = rec + L::k_codes(slot);
+            vp = rec + L::v_codes(c.page_shift, slot);
+            ks = rec + L::k_scales(c.page_shift, slot);
+            vs = rec + L::v_scales(c.page_shift, slot);
+        }
+        const uint32_t tile_code = TP == 1 ? i * 16 * L::code_bytes : 0, tile_scale = TP == 1 ? i * 16 * L::scale_bytes : 0;
+        load_words<HD>(kp + (at.code + tile_code), k.w[i]);
+        load_words<HD>(vp + (at.code + tile_code), v.w[i]);
+        k.scale[i] = ks[at.scale + tile_scale];
+        v.scale[i] = vs[at.scale + tile_scale];
+    }
+}
+
+// What load_chunk left to do for chunks at an end of lo..hi or of the pool: keys of a page
+// that is not there read as NaN, values outside lo..hi as zeros.
+template <int HD, int TP>
+__device__ __attribute__((always_inline)) inline void trim_chunk(const Cache &c, const Places<TP> &places,
+                                                                 uint32_t chunk, uint32_t lo, uint32_t hi, uint32_t n,
+                                                                 Codes<HD> &k, Codes<HD> &v) {
+#pragma unroll
+    for (uint32_t i = 0; i < kTiles; ++i) {
+        const uint32_t at = chunk * kChunk + 16 * i + n;
+        const bool in_pool = places.page[TP == 1 ? 0 : i] < c.pages;
+        const bool zero = at < lo || at > hi || !in_pool;
+        if (!in_pool) {
             k.scale[i] = 255;
-            v.scale[i] = 0;
+        }
+        v.scale[i] = zero ? 127u : v.scale[i];
+#pragma unroll
+        for (int s = 0; s < HD / 32; ++s) {
+            v.w[i][s] = zero ? 0u : v.w[i][s];
         }
     }
+}
+
+template <int TP>
+__device__ __attribute__((always_inline)) inline bool all_in_pool(const Cache &c, const Places<TP> &p) {
+    bool in = true;
+#pragma unroll
+    for (int i = 0; i < TP; ++i) {
+        in &= p.page[i] < c.pages;
+    }
+    return in;
 }
 
 // ---- the running softmax of a wave's queries ----------------------------------------------------
@@ -321,18 +370,14 @@ constexpr uint32_t kVStride = HD + 16;
 
 template <int HD, class V>
 __device__ __attribute__((always_inline)) inline void stage_values(uint16_t *lds, const Codes<HD> &v, uint32_t n,
-                                                                   uint32_t g, uint32_t chunk, uint32_t lo, uint32_t hi,
-                                                                   bool inside) {
+                                                                   uint32_t g) {
 #pragma unroll
     for (uint32_t i = 0; i < kTiles; ++i) {
-        // positions outside lo..hi, and NaN blocks (counted apart), are zeros
-        const uint32_t at = chunk * kChunk + 16 * i + n;
-        const bool zero = (!inside && (at < lo || at > hi)) || v.scale[i] == 255;
-        const float scale = zero ? 1.0f : kv4::scale_of(v.scale[i]);
+        const float scale = kv4::scale_of(v.scale[i]);
         uint16_t *row = lds + (16 * i + n) * kVStride<HD> + g * (HD / 4);
 #pragma unroll
         for (int s = 0; s < HD / 32; ++s) {
-            *reinterpret_cast<V *>(row + 8 * s) = mf::decode_as<V>(zero ? 0u : v.w[i][s], scale);
+            *reinterpret_cast<V *>(row + 8 * s) = mf::decode_as<V>(v.w[i][s], scale);
         }
     }
 }
@@ -455,12 +500,149 @@ __device__ inline f32x4 with_sink(const Params &a, uint32_t head, float b, f32x4
 }
 
 // ---- few queries: the waves of a workgroup share them and take the chunks in turn -----------------
-//
-// What bounds it: at long contexts the cache's bytes.  (Figures with the launch.)
-template <int HD, class T, int QT>
-__global__ __launch_bounds__(kThreads) void attention_split_kernel(Cache c, Batch b, Params a, Plan plan,
-                                                                   const T *__restrict__ q, T *__restrict__ out) {
+
+template <int HD, int QT, int QP>
+struct Wave {
+    State<HD, QT> st;
+    bf16x8 qf[QT][HD / 32][QP];
+    Query mine[QT];
+    uint32_t nan_blocks[QT];  // blocks of V (a bit each) that hold a NaN the query sees, by lane
+};
+
+// A wave's chunks from `chunk` on, every kWaves-th below `end`.  ODD false: it returns at the
+// first chunk with a scale byte of V outside the f16 path's (its number, or one past the
+// end); ODD true: it takes every chunk to the end on the bf16 path.  A loop of its own for each
+// keeps the running state in registers.
+template <int HD, class T, int QT, int TP, bool ODD>
+__device__ __attribute__((always_inline)) inline uint32_t walk(const Cache &c, const Params &a, const Block &k,
+                                                               const int32_t *table, uint32_t kv_head, uint32_t chunk,
+                                                               uint32_t end, Codes<HD> &kc, Codes<HD> &vc,
+                                                               Places<TP> here, uint16_t *lds, uint32_t n, uint32_t g,
+                                                               Wave<HD, QT, kQueryPlanes<T>> &w) {
     constexpr int NS = HD / 32, QP = kQueryPlanes<T>, PP = kWeightPlanes<T>;
+    const LaneOffsets<HD> at(n, g);
+    // the smallest last and the largest first position of the block's queries, for whole chunks
+    const uint32_t last_min = uint32_t(max(k.position0 + int32_t(k.query0 / a.group), 0));
+    const uint32_t first_max = a.window && k.hi + 1 > a.window ? k.hi + 1 - a.window : 0;
+    Places<TP> next = places_of<TP>(c, table, min(chunk + kWaves, end - 1), k.lo, k.hi);
+    while (true) {
+        const uint32_t c0 = chunk * kChunk;
+        const bool inside = c0 >= k.lo && c0 + kChunk - 1 <= k.hi;
+        const bool whole = c0 >= first_max && c0 + kChunk - 1 <= last_min;
+        if (!inside || !all_in_pool(c, here)) {
+            trim_chunk<HD, TP>(c, here, chunk, k.lo, k.hi, n, kc, vc);
+        }
+        if (!ODD) {
+            uint32_t far = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < kTiles; ++i) {
+                far = max(far, vc.scale[i] - kF16First);
+            }
+            if (__any(far > kF16Last - kF16First)) {
+                return chunk;
+            }
+        }
+        const uint32_t ahead = min(chunk + kWaves, end - 1);
+        Codes<HD> kn, vn;
+        load_chunk<HD, TP>(c, kv_head, next, ahead, k.lo, k.hi, at, kn, vn);
+        here = next;
+        next = places_of<TP>(c, table, min(chunk + 2 * kWaves, end - 1), k.lo, k.hi);
+
+        // S^T
+        f32x4 s[QT][kTiles];
+#pragma unroll
+        for (uint32_t i = 0; i < kTiles; ++i) {
+            const float scale = kv4::scale_of(kc.scale[i]);
+#pragma unroll
+            for (int ks = 0; ks < NS; ++ks) {
+                const bf16x8 kf = mf::decode_step(kc.w[i][ks], scale);
+#pragma unroll
+                for (int p = QP - 1; p >= 0; --p) {
+#pragma unroll
+                    for (int qi = 0; qi < QT; ++qi) {
+                        s[qi][i] = mf::mfma(kf, w.qf[qi][ks][p],
+                                            ks == 0 && p == QP - 1 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[qi][i]);
+                    }
+                }
+            }
+        }
+        if (ODD) {
+            // NaN blocks of a position, a bit each, behind its row (its lanes are n, n + 16,
+            // n + 32, n + 48); their values are zeros here
+#pragma unroll
+            for (uint32_t i = 0; i < kTiles; ++i) {
+                const bool nan = vc.scale[i] == 255;
+                const uint32_t bits = or_over_groups(nan ? 1u << (g * (HD / 4) / 32) : 0u);
+                if (g == 0) {
+                    lds[(16 * i + n) * kVStride<HD> + HD] = uint16_t(bits);
+                }
+                vc.scale[i] = nan ? 127u : vc.scale[i];
+#pragma unroll
+                for (int x = 0; x < NS; ++x) {
+                    vc.w[i][x] = nan ? 0u : vc.w[i][x];
+                }
+            }
+            stage_values<HD, bf16x8>(lds, vc, n, g);
+        } else {
+            stage_values<HD, f16x8>(lds, vc, n, g);
+        }
+#pragma unroll
+        for (int qi = 0; qi < QT; ++qi) {
+            softmax_step<HD, QT>(s[qi], w.st, qi, w.mine[qi], whole, chunk, g, a.c);
+        }
+        __builtin_amdgcn_wave_barrier();
+        asm volatile("" ::: "memory");
+        if (ODD) {
+            weigh_values<HD, bf16x8, 3, QT>(lds, s, w.st, n, g);
+#pragma unroll
+            for (uint32_t i = 0; i < kTiles; ++i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t bits = lds[(16 * i + 4 * g + j) * kVStride<HD> + HD];
+                    const int32_t p = int32_t(c0 + 16 * i + 4 * g) + j;
+#pragma unroll
+                    for (int qi = 0; qi < QT; ++qi) {
+                        w.nan_blocks[qi] |= p >= w.mine[qi].first && p <= w.mine[qi].last ? bits : 0u;
+                    }
+                }
+            }
+        } else {
+            weigh_values<HD, f16x8, PP, QT>(lds, s, w.st, n, g);
+        }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_wave_barrier();
+        chunk += kWaves;
+        if (chunk >= end) {
+            return chunk;
+        }
+        kc = kn;
+        vc = vn;
+    }
+}
+
+// The walk on the bf16 path, with a copy of the state, so that the other walk's stays in
+// registers of its own.
+template <int HD, class T, int QT, int TP>
+__device__ __attribute__((always_inline)) inline void walk_odd(const Cache &c, const Params &a, const Block &k,
+                                                   const int32_t *table, uint32_t kv_head, uint32_t chunk,
+                                                   uint32_t end, uint16_t *lds, uint32_t n, uint32_t g,
+                                                   Wave<HD, QT, kQueryPlanes<T>> &w) {
+    const Places<TP> here = places_of<TP>(c, table, chunk, k.lo, k.hi);
+    Codes<HD> kc, vc;
+    load_chunk<HD, TP>(c, kv_head, here, chunk, k.lo, k.hi, LaneOffsets<HD>(n, g), kc, vc);
+    Wave<HD, QT, kQueryPlanes<T>> mine = w;
+    walk<HD, T, QT, TP, true>(c, a, k, table, kv_head, chunk, end, kc, vc, here, lds, n, g, mine);
+    w = mine;
+}
+
+// What bounds it: at long contexts the cache's bytes.  (Figures with the launch.)
+// Waves per SIMD that the kernel's registers leave room for.
+template <int HD, class T, int QT>
+constexpr int kResident = QT == 2 ? (HD == 64 ? 2 : 1) : HD == 128 ? 2 : std::is_same<T, float>::value ? 3 : 4;
+
+template <int HD, class T, int QT, int TP>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kResident<HD, T, QT>))) void
+attention_split_kernel(Cache c, Batch b, Params a, Plan plan, const T *__restrict__ q, T *__restrict__ out) {
     constexpr uint32_t kQueries = 16 * QT, kOStride = HD + 4;
     constexpr uint32_t kVWave = kChunk * kVStride<HD>;  // 16-bit values of one wave
     union Shared {
@@ -472,9 +654,8 @@ __global__ __launch_bounds__(kThreads) void attention_split_kernel(Cache c, Batc
     };
     __shared__ __attribute__((aligned(16))) Shared sh;
 
-    const uint32_t run = blockIdx.x % plan.splits;
-    const uint32_t kv_head = blockIdx.x / plan.splits % c.kv_heads, index = blockIdx.x / plan.splits / c.kv_heads;
-    const Block k = block_of(b, a, kQueries, index);
+    const uint32_t run = blockIdx.z, kv_head = blockIdx.y;
+    const Block k = block_of(b, a, kQueries, blockIdx.x);
     if (!k.exists) {
         return;
     }
@@ -484,120 +665,42 @@ __global__ __launch_bounds__(kThreads) void attention_split_kernel(Cache c, Batc
         return;
     }
     const uint32_t wave = __builtin_amdgcn_readfirstlane(t / 64), lane = t % 64, n = lane % 16, g = lane / 16;
-
-    State<HD, QT> st;
-    bf16x8 qf[QT][NS][QP];
-    Query mine[QT];
-    uint32_t nan_blocks[QT];
-#pragma unroll
-    for (int qi = 0; qi < QT; ++qi) {
-        const uint32_t query = k.query0 + 16 * qi + n, token = query / a.group;
-        const bool there = query < k.rows * a.group;
-        const int32_t position = k.position0 + int32_t(token);
-        mine[qi].last = there ? position : -1;
-        mine[qi].first = a.window && position + 1 > int32_t(a.window) ? position + 1 - int32_t(a.window) : 0;
-        const uint32_t row = k.row0 + (there ? token : 0u);
-        const uint32_t head = kv_head * a.group + (there ? query % a.group : 0u);
-        load_query<HD, T>(q + (size_t(row) * a.heads + head) * HD, g, a.negate, qf[qi]);
-        st.b[qi] = -INFINITY;
-        st.l[qi] = 0.0f;
-        nan_blocks[qi] = 0;
-#pragma unroll
-        for (int mt = 0; mt < HD / 16; ++mt) {
-            st.o[qi][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
-        }
-    }
-
-    uint16_t *const lds = sh.v[wave];
     const int32_t *const table = b.table + size_t(k.sequence) * b.stride;
     const uint32_t end = k.first_chunk + min(k.chunks, (run + 1) * plan.run);
-    uint32_t chunk = k.first_chunk + run * plan.run + wave;
-    if (chunk < end) {
-        Codes<HD> kc, vc;
-        load_chunk<HD>(c, kv_head, pages_of(c, table, chunk, k.lo, k.hi), chunk, k.lo, k.hi, n, g, kc, vc);
-        Pages next = pages_of(c, table, min(chunk + kWaves, end - 1), k.lo, k.hi);
-        // the smallest `last` and the largest `first` of the block's queries, for whole chunks
-        const uint32_t last_min = uint32_t(max(k.position0 + int32_t(k.query0 / a.group), 0));
-        const uint32_t first_max = a.window && k.hi + 1 > a.window ? k.hi + 1 - a.window : 0;
-        while (true) {
-            const uint32_t ahead = min(chunk + kWaves, end - 1);
-            Codes<HD> kn, vn;
-            load_chunk<HD>(c, kv_head, next, ahead, k.lo, k.hi, n, g, kn, vn);
-            next = pages_of(c, table, min(chunk + 2 * kWaves, end - 1), k.lo, k.hi);
+    const uint32_t first = k.first_chunk + run * plan.run + wave;
 
-            const uint32_t c0 = chunk * kChunk;
-            const bool inside = c0 >= k.lo && c0 + kChunk - 1 <= k.hi;
-            const bool whole = c0 >= first_max && c0 + kChunk - 1 <= last_min;
-            // S^T
-            f32x4 s[QT][kTiles];
+    Wave<HD, QT, kQueryPlanes<T>> w;
+    Places<TP> here{};
+    Codes<HD> kc, vc;
+    if (first < end) {
+        here = places_of<TP>(c, table, first, k.lo, k.hi);
+        load_chunk<HD, TP>(c, kv_head, here, first, k.lo, k.hi, LaneOffsets<HD>(n, g), kc, vc);
+    }
 #pragma unroll
-            for (uint32_t i = 0; i < kTiles; ++i) {
-                const float scale = kv4::scale_of(kc.scale[i]);
+    for (int qi = 0; qi < QT; ++qi) {
+        const uint32_t query = k.query0 + 16 * qi + n, token = k.rows == 1 ? 0u : query / a.group;
+        const bool there = query < k.rows * a.group;
+        const int32_t position = k.position0 + int32_t(token);
+        w.mine[qi].last = there ? position : -1;
+        w.mine[qi].first = a.window && position + 1 > int32_t(a.window) ? position + 1 - int32_t(a.window) : 0;
+        const uint32_t row = k.row0 + (there ? token : 0u);
+        const uint32_t head = kv_head * a.group + (there ? query - token * a.group : 0u);
+        load_query<HD, T>(q + (size_t(row) * a.heads + head) * HD, g, a.negate, w.qf[qi]);
+        w.st.b[qi] = -INFINITY;
+        w.st.l[qi] = 0.0f;
+        w.nan_blocks[qi] = 0;
 #pragma unroll
-                for (int ks = 0; ks < NS; ++ks) {
-                    const bf16x8 kf = mf::decode_step(kc.w[i][ks], scale);
-#pragma unroll
-                    for (int p = QP - 1; p >= 0; --p) {
-#pragma unroll
-                        for (int qi = 0; qi < QT; ++qi) {
-                            s[qi][i] = mf::mfma(kf, qf[qi][ks][p],
-                                                ks == 0 && p == QP - 1 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[qi][i]);
-                        }
-                    }
-                }
-            }
-            // V: f16 unless a scale byte leaves its range
-            bool odd = false;
-#pragma unroll
-            for (uint32_t i = 0; i < kTiles; ++i) {
-                const uint32_t at = c0 + 16 * i + n;
-                odd |= (vc.scale[i] != 0 && vc.scale[i] - 104u > 36u) && (inside || (at >= k.lo && at <= k.hi));
-            }
-            const bool f16 = !__any(odd);
-            if (f16) {
-                stage_values<HD, f16x8>(lds, vc, n, g, chunk, k.lo, k.hi, inside);
-            } else {
-                stage_values<HD, bf16x8>(lds, vc, n, g, chunk, k.lo, k.hi, inside);
-                // NaN blocks of a position, a bit each, behind its row: lanes of one position are n, n + 16, n + 32, n + 48
-#pragma unroll
-                for (uint32_t i = 0; i < kTiles; ++i) {
-                    const uint32_t bits = or_over_groups(vc.scale[i] == 255 ? 1u << (g * (HD / 4) / 32) : 0u);
-                    if (g == 0) {
-                        lds[(16 * i + n) * kVStride<HD> + HD] = uint16_t(bits);
-                    }
-                }
-            }
-#pragma unroll
-            for (int qi = 0; qi < QT; ++qi) {
-                softmax_step<HD, QT>(s[qi], st, qi, mine[qi], whole, chunk, g, a.c);
-            }
-            __builtin_amdgcn_wave_barrier();
-            asm volatile("" ::: "memory");
-            if (f16) {
-                weigh_values<HD, f16x8, PP, QT>(lds, s, st, n, g);
-            } else {
-                weigh_values<HD, bf16x8, 3, QT>(lds, s, st, n, g);
-#pragma unroll
-                for (uint32_t i = 0; i < kTiles; ++i) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t bits = lds[(16 * i + 4 * g + j) * kVStride<HD> + HD];
-                        const int32_t at = int32_t(c0 + 16 * i + 4 * g) + j;
-#pragma unroll
-                        for (int qi = 0; qi < QT; ++qi) {
-                            nan_blocks[qi] |= at >= mine[qi].first && at <= mine[qi].last ? bits : 0u;
-                        }
-                    }
-                }
-            }
-            asm volatile("" ::: "memory");
-            __builtin_amdgcn_wave_barrier();
-            chunk += kWaves;
-            if (chunk >= end) {
-                break;
-            }
-            kc = kn;
-            vc = vn;
+        for (int mt = 0; mt < HD / 16; ++mt) {
+            w.st.o[qi][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+    if (first < end) {
+        uint16_t *const lds = sh.v[wave];
+        const uint32_t at = walk<HD, T, QT, TP, false>(c, a, k, table, kv_head, first, end, kc, vc, here, lds, n, g, w);
+        if (at < end) {
+            Wave<HD, QT, kQueryPlanes<T>> copy = w;  // (the state itself stays in registers)
+            walk_odd<HD, T, QT, TP>(c, a, k, table, kv_head, at, end, lds, n, g, copy);
+            w = copy;
         }
     }
 
@@ -605,15 +708,15 @@ __global__ __launch_bounds__(kThreads) void attention_split_kernel(Cache c, Batc
     __syncthreads();
 #pragma unroll
     for (int qi = 0; qi < QT; ++qi) {
-        const uint32_t poison = or_over_groups(nan_blocks[qi]);
-        const float l = sum_over_groups(st.l[qi]);
+        const uint32_t poison = or_over_groups(w.nan_blocks[qi]);
+        const float l = sum_over_groups(w.st.l[qi]);
         if (g == 0) {
-            sh.join.b[wave][16 * qi + n] = st.b[qi];
+            sh.join.b[wave][16 * qi + n] = w.st.b[qi];
             sh.join.l[wave][16 * qi + n] = l;
         }
 #pragma unroll
         for (int mt = 0; mt < HD / 16; ++mt) {
-            f32x4 o = st.o[qi][mt];
+            f32x4 o = w.st.o[qi][mt];
             if (poison >> (mt / 2) & 1) {
                 o = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
             }
@@ -804,7 +907,7 @@ int run_attention(ttl_ctx *ctx, const ttl_kv4_cache *cache, const ttl_kv4_batch 
     TTL_REQUIRE(cut.workspace == 0 || (uintptr_t(workspace) & 255) == 0, TTL_ERR_INVALID,
                 "%s: the workspace must be 256-byte aligned", what);
     const uint64_t groups = uint64_t(cut.plan.blocks) * cache->kv_heads * cut.plan.splits;
-    TTL_REQUIRE(groups <= 0x7fffffffu && uint64_t(batch->tokens) * attention->heads <= 0x7fffffffu, TTL_ERR_SHAPE,
+    TTL_REQUIRE(groups * kThreads <= 0xffffffffu && uint64_t(batch->tokens) * attention->heads <= 0x7fffffffu, TTL_ERR_SHAPE,
                 "%s: %u tokens of %u heads are too many for one call", what, batch->tokens, attention->heads);
     TTL_HIP(hipSetDevice(ctx->device));
     const Cache c = kv4::view(cache);
@@ -829,10 +932,20 @@ int run_attention(ttl_ctx *ctx, const ttl_kv4_cache *cache, const ttl_kv4_batch 
         using T = decltype(zero);
         const T *qt = static_cast<const T *>(q);
         T *ot = static_cast<T *>(out);
+        const dim3 grid(p.blocks, c.kv_heads, p.splits);
+        const bool big = c.page_shift >= 6;
+        const auto split = [&](auto tiles) {
+            constexpr int QT = decltype(tiles)::value;
+            if (big) {
+                attention_split_kernel<HD, T, QT, 1><<<grid, kThreads, 0, ctx->stream>>>(c, b, a, p, qt, ot);
+            } else {
+                attention_split_kernel<HD, T, QT, 4><<<grid, kThreads, 0, ctx->stream>>>(c, b, a, p, qt, ot);
+            }
+        };
         if (cut.tiles == 1) {
-            attention_split_kernel<HD, T, 1><<<uint32_t(groups), kThreads, 0, ctx->stream>>>(c, b, a, p, qt, ot);
+            split(std::integral_constant<int, 1>());
         } else {
-            attention_split_kernel<HD, T, 2><<<uint32_t(groups), kThreads, 0, ctx->stream>>>(c, b, a, p, qt, ot);
+            split(std::integral_constant<int, 2>());
         }
         if (p.splits > 1) {
             attention_join_kernel<HD, T><<<ttl::blocks_for(size_t(b.tokens) * a.heads, kWaves), kThreads, 0,
