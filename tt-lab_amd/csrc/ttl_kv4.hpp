@@ -25,6 +25,16 @@ int check(const ttl_kv4_cache *cache, const ttl_kv4_batch *batch, const char *wh
 Cache view(const ttl_kv4_cache *cache);
 Batch view(const ttl_kv4_batch *batch);
 
+// An entry of the call's index arrays, which nothing writes while a kernel runs: a scalar load
+// where the index is uniform, also in a kernel that stores.
+__host__ __device__ inline int32_t entry(const int32_t *p, size_t i) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    return reinterpret_cast<const __attribute__((address_space(4))) int32_t *>(reinterpret_cast<uintptr_t>(p))[i];
+#else
+    return p[i];
+#endif
+}
+
 // What a row of the call's arrays stands for.
 enum RowKind : uint32_t {
     kPadding,  // neither read nor written
@@ -41,7 +51,7 @@ __host__ __device__ inline uint32_t sequence_of(const Batch &b, uint32_t row) {
     uint32_t lo = 0, hi = b.sequences;
     while (hi - lo > 1) {
         const uint32_t mid = lo + (hi - lo) / 2;
-        if (b.starts[mid] <= int32_t(row)) {
+        if (entry(b.starts, mid) <= int32_t(row)) {
             lo = mid;
         } else {
             hi = mid;
@@ -55,13 +65,13 @@ __host__ __device__ inline Row row_of(const Batch &b, uint32_t row) {
     int32_t end = int32_t(row) + 1;
     if (b.starts) {
         r.sequence = sequence_of(b, row);
-        end = b.starts[r.sequence + 1];
-        if (b.starts[r.sequence] > int32_t(row) || end <= int32_t(row)) {
+        end = entry(b.starts, r.sequence + 1);
+        if (entry(b.starts, r.sequence) > int32_t(row) || end <= int32_t(row)) {
             r.kind = kPadding;
             return r;
         }
     }
-    const int32_t length = b.lengths[r.sequence];
+    const int32_t length = entry(b.lengths, r.sequence);
     const int64_t position = int64_t(length) - (int64_t(end) - int64_t(row));
     if (length <= 0 || position < 0) {
         r.kind = kIdle;
@@ -73,8 +83,9 @@ __host__ __device__ inline Row row_of(const Batch &b, uint32_t row) {
 }
 
 // The page of a position below max_length; false where the table names none of the pool.
-__host__ __device__ inline bool page_of(const Cache &c, const Batch &b, uint32_t sequence, uint32_t position, uint32_t &page) {
-    page = uint32_t(b.table[size_t(sequence) * b.stride + (position >> c.page_shift)]);
+__host__ __device__ inline bool page_of(const Cache &c, const Batch &b, uint32_t sequence, uint32_t position,
+                                        uint32_t &page) {
+    page = uint32_t(entry(b.table, size_t(sequence) * b.stride + (position >> c.page_shift)));
     return page < c.pages;
 }
 

@@ -18,9 +18,9 @@
 // weights never leave their registers.
 //
 // Numerics: K and bf16 queries are exact in bf16, f32 queries three bf16 planes (24 bits).  The
-// weights, at most 1 and held times 2^15, are rounded to f16 for a bf16 output (2^-11, an eighth
-// of the output's own rounding) and to two f16 planes for an f32 one (2^-22; weights below
-// 2^-29 of the largest lose more of themselves, 2^-40 of the largest).  V is exact in f16 where
+// weights, relative to a large one held as 2^11, are rounded to f16 for a bf16 output (2^-11, an
+// eighth of the output's own rounding) and to two f16 planes for an f32 one (2^-22; weights
+// below 2^-25 of the large one lose more of themselves, 2^-36 of it).  V is exact in f16 where
 // its scale bytes are 104..140 (subnormals included: the matrix cores keep them); a chunk with
 // another one takes V as bf16, exact for every byte, and three bf16 planes of the weights.
 // Maxima, sums and outputs are f32.
@@ -48,7 +48,7 @@ constexpr uint32_t kChunk = 64, kTiles = kChunk / 16;
 constexpr uint32_t kWaves = 4, kThreads = kWaves * 64;
 constexpr float kLog2e = 0x1.715476p+0f, kLog2eLo = 0x1.4ae0cp-26f;  // log2 e = their sum
 constexpr uint32_t kF16First = 104, kF16Last = 140;                  // scale bytes of V on the f16 path
-constexpr float kWeightShift = 15.0f;                               // weights are held times 2^15
+constexpr float kWeightShift = 11.0f;                               // weights are held times 2^11
 
 struct Params {
     const float *sinks;
@@ -58,12 +58,18 @@ struct Params {
     bool negate;  // the scale is negative: the queries change their sign instead
 };
 
-// How a call is cut: blocks of `queries` queries of a sequence and key/value head, each
-// block's chunks in runs of `run` chunks, `splits` at most.
+// How a call is cut.  A block is up to `queries` queries of a sequence and key/value head; its
+// chunks count in units of kWaves, one chunk a wave.  The units of all blocks in a row are
+// divided evenly among `shares` workgroups per key/value head, whatever the lengths are: a share
+// takes the end of one block, whole ones, and the beginning of another.  A block that one
+// share has whole is written by it; of the others every share leaves its part in `o` and `bl`
+// (place 1 where it holds the block's beginning, 0 elsewhere) for the join.
 struct Plan {
-    uint32_t queries, blocks, run, splits;
-    float *o;      // [split][row][head][HD], where a block has more than one run
-    float2 *bl;    // [split][row][head]: offset, sum
+    uint32_t queries, blocks, shares;
+    bool single;   // no block has more than one unit: a share is a block, nothing is joined
+    float *o;      // [kv head][share][2][queries][HD]
+    float2 *bl;    // [kv head][share][2][queries]: offset, sum
+    uint2 *span;   // [block]: its first and last share
 };
 
 // ---- which queries and positions a block has -----------------------------------------------
@@ -75,10 +81,11 @@ struct Block {
     uint32_t first_chunk, chunks;      // none: no row of the block sees a position
     uint32_t lo, hi;                   // the positions that its rows see
     bool exists, bad;
+    __device__ uint32_t units() const { return (chunks + kWaves - 1) / kWaves; }
 };
 
 __device__ inline Block block_span(const Batch &b, const Params &a, uint32_t queries, Block k) {
-    const int32_t length = b.lengths[k.sequence];
+    const int32_t length = kv4::entry(b.lengths, k.sequence);
     k.position0 = length - int32_t(k.rows);
     k.bad = length > 0 && uint32_t(length) > b.max_length;
     const uint32_t last = min(k.query0 + queries, k.rows * a.group) - 1;
@@ -109,7 +116,7 @@ __device__ inline Block block_of(const Batch &b, const Params &a, uint32_t queri
         uint32_t lo = 0, hi = b.sequences;
         while (hi - lo > 1) {
             const uint32_t mid = lo + (hi - lo) / 2;
-            const uint32_t s = uint32_t(max(b.starts[mid], 0));
+            const uint32_t s = uint32_t(max(kv4::entry(b.starts, mid), 0));
             if (uint64_t(s) * a.group / queries + mid <= index) {
                 lo = mid;
             } else {
@@ -117,8 +124,8 @@ __device__ inline Block block_of(const Batch &b, const Params &a, uint32_t queri
             }
         }
         k.sequence = lo;
-        k.row0 = min(uint32_t(max(b.starts[lo], 0)), b.tokens);
-        const uint32_t end = min(uint32_t(max(b.starts[lo + 1], 0)), b.tokens);
+        k.row0 = min(uint32_t(max(kv4::entry(b.starts, lo), 0)), b.tokens);
+        const uint32_t end = min(uint32_t(max(kv4::entry(b.starts, lo + 1), 0)), b.tokens);
         k.rows = end > k.row0 ? end - k.row0 : 0;
         const uint64_t base = uint64_t(k.row0) * a.group / queries + lo;
         if (index < base) {
@@ -173,7 +180,7 @@ __device__ __attribute__((always_inline)) inline Places<TP> places_of(const Cach
 #pragma unroll
     for (uint32_t i = 0; i < TP; ++i) {
         const uint32_t tile = TP == 1 ? chunk * kTiles : min(max(chunk * kTiles + i, lo / 16), hi / 16);
-        p.page[i] = uint32_t(table[tile >> (c.page_shift - 4)]);
+        p.page[i] = uint32_t(kv4::entry(table, tile >> (c.page_shift - 4)));
     }
     return p;
 }
@@ -249,7 +256,7 @@ __device__ __attribute__((always_inline)) inline bool all_in_pool(const Cache &c
 
 template <int HD, int QT>
 struct State {
-    float b[QT];  // offset: c x the largest score - 15; weights are 2^(c s - b)
+    float b[QT];  // offset: c x a large score - 11; weights are 2^(c s - b), 2^15 at most
     float l[QT];  // the lane's share of their sum
     f32x4 o[QT][HD / 16];  // O^T: dims 16 mt + 4g + i of column n
 };
@@ -278,7 +285,9 @@ struct Query {
     int32_t first, last;
 };
 
-// Scores to weights: masks, the new maximum, the rescaling of what is there.
+// Scores to weights.  The offset follows the largest score lazily: it is set anew (and what is
+// there rescaled) only when a lane's 16 weights pass 2^15 together, before which none leaves
+// the f16 range, or before any score was seen (its weights are then infinite).
 template <int HD, int QT>
 __device__ __attribute__((always_inline)) inline void softmax_step(f32x4 (&s)[kTiles], State<HD, QT> &st, int qi,
                                                                    const Query &q, bool whole, uint32_t chunk,
@@ -293,18 +302,32 @@ __device__ __attribute__((always_inline)) inline void softmax_step(f32x4 (&s)[kT
             }
         }
     }
-    float m = s[0][0];
+    const auto weigh = [&](float base, f32x4 (&p)[kTiles]) __attribute__((always_inline)) {
+        float sum = 0.0f;
 #pragma unroll
-    for (uint32_t i = 0; i < kTiles; ++i) {
+        for (uint32_t i = 0; i < kTiles; ++i) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            m = fmaxf(m, s[i][j]);
+            for (int j = 0; j < 4; ++j) {
+                p[i][j] = __builtin_amdgcn_exp2f(fmaf(s[i][j], c, -base));
+                sum += p[i][j];
+            }
         }
-    }
-    m = max_over_groups(m);
-    // fmaxf drops NaN scores; their weights are NaN all the same
-    const float b = fmaxf(st.b[qi], m == -INFINITY ? m : fmaf(m, c, -kWeightShift));
-    if (__any(b != st.b[qi])) {
+        return sum;
+    };
+    f32x4 p[kTiles];
+    float sum = weigh(st.b[qi], p);
+    if (__any(!(sum <= 0x1p15f))) {
+        float m = s[0][0];
+#pragma unroll
+        for (uint32_t i = 0; i < kTiles; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                m = fmaxf(m, s[i][j]);
+            }
+        }
+        m = max_over_groups(m);
+        // fmaxf drops NaN scores; their weights are NaN all the same
+        const float b = fmaxf(st.b[qi], m == -INFINITY ? m : fmaf(m, c, -kWeightShift));
         const float keep = b == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st.b[qi] - b);
         st.b[qi] = b;
         st.l[qi] *= keep;
@@ -315,19 +338,13 @@ __device__ __attribute__((always_inline)) inline void softmax_step(f32x4 (&s)[kT
                 st.o[qi][mt][j] *= keep;
             }
         }
-    }
-    const float base = b == -INFINITY ? 0.0f : b;
-    float sum = 0.0f;
-#pragma unroll
-    for (uint32_t i = 0; i < kTiles; ++i) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(s[i][j], c, -base));
-            s[i][j] = p;
-            sum += p;
-        }
+        sum = weigh(b == -INFINITY ? 0.0f : b, p);
     }
     st.l[qi] += sum;
+#pragma unroll
+    for (uint32_t i = 0; i < kTiles; ++i) {
+        s[i] = p[i];
+    }
 }
 
 template <class V>
@@ -398,27 +415,47 @@ __device__ __attribute__((always_inline)) inline V value_fragment(const uint16_t
 template <int HD, class V, int PP, int QT>
 __device__ __attribute__((always_inline)) inline void weigh_values(const uint16_t *lds, const f32x4 (&s)[QT][kTiles],
                                                                    State<HD, QT> &st, uint32_t n, uint32_t g) {
+    constexpr int kSteps = int(kTiles) / 2, kBatch = 4;  // fragments requested together, a batch ahead
+    constexpr int kFragments = kSteps * (HD / 16);
+    const auto fragment = [&](int f) __attribute__((always_inline)) {
+        return value_fragment<HD, V>(lds, f / (HD / 16), f % (HD / 16), n, g);
+    };
+    V a[2][kBatch];
 #pragma unroll
-    for (int h = 0; h < int(kTiles) / 2; ++h) {
-        V p[QT][PP];
+    for (int f = 0; f < kBatch; ++f) {
+        a[0][f] = fragment(f);
+    }
+    V p[QT][PP];
 #pragma unroll
-        for (int qi = 0; qi < QT; ++qi) {
-            float x[8];
+    for (int f0 = 0; f0 < kFragments; f0 += kBatch) {
+        const int h = f0 / (HD / 16);
+        if (f0 % (HD / 16) == 0) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x[j] = s[qi][2 * h][j];
-                x[4 + j] = s[qi][2 * h + 1][j];
+            for (int qi = 0; qi < QT; ++qi) {
+                float x[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    x[j] = s[qi][2 * h][j];
+                    x[4 + j] = s[qi][2 * h + 1][j];
+                }
+                split<V, PP>(x, p[qi]);
             }
-            split<V, PP>(x, p[qi]);
         }
+        if (f0 + kBatch < kFragments) {
 #pragma unroll
-        for (int mt = 0; mt < HD / 16; ++mt) {
-            const V a = value_fragment<HD, V>(lds, h, mt, n, g);
+            for (int f = 0; f < kBatch; ++f) {
+                a[(f0 / kBatch + 1) % 2][f] = fragment(f0 + kBatch + f);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int k = PP - 1; k >= 0; --k) {
+        for (int k = PP - 1; k >= 0; --k) {
+#pragma unroll
+            for (int f = 0; f < kBatch; ++f) {
+                const int mt = (f0 + f) % (HD / 16);
 #pragma unroll
                 for (int qi = 0; qi < QT; ++qi) {
-                    st.o[qi][mt] = mf::mfma(a, p[qi][k], st.o[qi][mt]);
+                    st.o[qi][mt] = mf::mfma(a[f0 / kBatch % 2][f], p[qi][k], st.o[qi][mt]);
                 }
             }
         }
@@ -426,25 +463,6 @@ __device__ __attribute__((always_inline)) inline void weigh_values(const uint16_
 }
 
 // ---- queries -------------------------------------------------------------------------------------
-
-__device__ inline void load8(const float *p, float (&v)[8]) {
-    const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
-    v[0] = a.x;
-    v[1] = a.y;
-    v[2] = a.z;
-    v[3] = a.w;
-    v[4] = b.x;
-    v[5] = b.y;
-    v[6] = b.z;
-    v[7] = b.w;
-}
-__device__ inline void load8(const __bf16 *p, float (&v)[8]) {
-    const bf16x8 x = *reinterpret_cast<const bf16x8 *>(p);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        v[i] = float(x[i]);
-    }
-}
 
 __device__ inline void store4(float *p, const f32x4 &v) {
     *reinterpret_cast<f32x4 *>(p) = v;
@@ -462,19 +480,37 @@ constexpr int kWeightPlanes = std::is_same<T, float>::value ? 2 : 1;
 // The lane's query as B operand of K step s: dims g HD/4 + 8s .., in K's order.  A value that
 // is not finite makes every score NaN.
 template <int HD, class T>
-__device__ __attribute__((always_inline)) inline void load_query(const T *q, uint32_t g, bool negate,
-                                                                 bf16x8 (&out)[HD / 32][kQueryPlanes<T>]) {
+struct RawQuery {
+    static constexpr int kLoads = HD / 4 * int(sizeof(T)) / 16;
+    mf::u32x4 raw[kLoads];
+    __device__ __attribute__((always_inline)) inline void load(const T *q, uint32_t g) {
 #pragma unroll
-    for (int s = 0; s < HD / 32; ++s) {
-        float v[8];
-        load8(q + g * (HD / 4) + 8 * s, v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            v[e] = __builtin_isfinite(v[e]) ? (negate ? -v[e] : v[e]) : __builtin_nanf("");
+        for (int i = 0; i < kLoads; ++i) {
+            raw[i] = reinterpret_cast<const mf::u32x4 *>(q + g * (HD / 4))[i];
         }
-        split<bf16x8, kQueryPlanes<T>>(v, out[s]);
     }
-}
+    __device__ __attribute__((always_inline)) inline float value(int s, int e) const {
+        if constexpr (std::is_same<T, float>::value) {
+            return __uint_as_float(raw[2 * s + e / 4][e % 4]);
+        } else {
+            const uint32_t w = raw[s][e / 2];
+            return __uint_as_float(e % 2 ? w & 0xffff0000u : w << 16);
+        }
+    }
+    __device__ __attribute__((always_inline)) inline void planes(bool negate,
+                                                                 bf16x8 (&out)[HD / 32][kQueryPlanes<T>]) const {
+#pragma unroll
+        for (int s = 0; s < HD / 32; ++s) {
+            float v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[e] = value(s, e);
+                v[e] = __builtin_isfinite(v[e]) ? (negate ? -v[e] : v[e]) : __builtin_nanf("");
+            }
+            split<bf16x8, kQueryPlanes<T>>(v, out[s]);
+        }
+    }
+};
 
 // The output of sums o and l at offset b, with the head's sink in the denominator.
 __device__ inline f32x4 with_sink(const Params &a, uint32_t head, float b, f32x4 o, float l) {
@@ -517,14 +553,14 @@ template <int HD, class T, int QT, int TP, bool ODD>
 __device__ __attribute__((always_inline)) inline uint32_t walk(const Cache &c, const Params &a, const Block &k,
                                                                const int32_t *table, uint32_t kv_head, uint32_t chunk,
                                                                uint32_t end, Codes<HD> &kc, Codes<HD> &vc,
-                                                               Places<TP> here, uint16_t *lds, uint32_t n, uint32_t g,
+                                                               Places<TP> here, Places<TP> next, uint16_t *lds,
+                                                               uint32_t n, uint32_t g,
                                                                Wave<HD, QT, kQueryPlanes<T>> &w) {
     constexpr int NS = HD / 32, QP = kQueryPlanes<T>, PP = kWeightPlanes<T>;
     const LaneOffsets<HD> at(n, g);
     // the smallest last and the largest first position of the block's queries, for whole chunks
     const uint32_t last_min = uint32_t(max(k.position0 + int32_t(k.query0 / a.group), 0));
     const uint32_t first_max = a.window && k.hi + 1 > a.window ? k.hi + 1 - a.window : 0;
-    Places<TP> next = places_of<TP>(c, table, min(chunk + kWaves, end - 1), k.lo, k.hi);
     while (true) {
         const uint32_t c0 = chunk * kChunk;
         const bool inside = c0 >= k.lo && c0 + kChunk - 1 <= k.hi;
@@ -544,9 +580,9 @@ __device__ __attribute__((always_inline)) inline uint32_t walk(const Cache &c, c
         }
         const uint32_t ahead = min(chunk + kWaves, end - 1);
         Codes<HD> kn, vn;
-        load_chunk<HD, TP>(c, kv_head, next, ahead, k.lo, k.hi, at, kn, vn);
         here = next;
         next = places_of<TP>(c, table, min(chunk + 2 * kWaves, end - 1), k.lo, k.hi);
+        load_chunk<HD, TP>(c, kv_head, here, ahead, k.lo, k.hi, at, kn, vn);
 
         // S^T
         f32x4 s[QT][kTiles];
@@ -631,51 +667,53 @@ __device__ __attribute__((always_inline)) inline void walk_odd(const Cache &c, c
     Codes<HD> kc, vc;
     load_chunk<HD, TP>(c, kv_head, here, chunk, k.lo, k.hi, LaneOffsets<HD>(n, g), kc, vc);
     Wave<HD, QT, kQueryPlanes<T>> mine = w;
-    walk<HD, T, QT, TP, true>(c, a, k, table, kv_head, chunk, end, kc, vc, here, lds, n, g, mine);
+    const Places<TP> next = places_of<TP>(c, table, min(chunk + kWaves, end - 1), k.lo, k.hi);
+    walk<HD, T, QT, TP, true>(c, a, k, table, kv_head, chunk, end, kc, vc, here, next, lds, n, g, mine);
     w = mine;
 }
 
 // What bounds it: at long contexts the cache's bytes.  (Figures with the launch.)
 // Waves per SIMD that the kernel's registers leave room for.
 template <int HD, class T, int QT>
-constexpr int kResident = QT == 2 ? (HD == 64 ? 2 : 1) : HD == 128 ? 2 : std::is_same<T, float>::value ? 3 : 4;
+constexpr int kResident = QT == 2 ? (HD == 64 ? 2 : 1) : HD == 128 ? 2 : 3;
 
+template <int HD, int QT>
+union Shared {
+    static constexpr uint32_t kOStride = HD + 4;
+    uint16_t v[kWaves][kChunk * kVStride<HD>];
+    struct {
+        float o[kWaves][16 * QT][kOStride];
+        float b[kWaves][16 * QT], l[kWaves][16 * QT];
+    } join;
+    struct {
+        uint32_t sum[kWaves];
+        uint32_t block, first;  // the share's first block, and that block's first unit
+    } scan;
+};
+
+// Units [from, to) of a block: the waves take its chunks in turn, and their states are joined.
+// place < 0: the block is whole, its outputs are written; else the place of the share's part.
 template <int HD, class T, int QT, int TP>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kResident<HD, T, QT>))) void
-attention_split_kernel(Cache c, Batch b, Params a, Plan plan, const T *__restrict__ q, T *__restrict__ out) {
-    constexpr uint32_t kQueries = 16 * QT, kOStride = HD + 4;
-    constexpr uint32_t kVWave = kChunk * kVStride<HD>;  // 16-bit values of one wave
-    union Shared {
-        uint16_t v[kWaves][kVWave];
-        struct {
-            float o[kWaves][kQueries][kOStride];
-            float b[kWaves][kQueries], l[kWaves][kQueries];
-        } join;
-    };
-    __shared__ __attribute__((aligned(16))) Shared sh;
-
-    const uint32_t run = blockIdx.z, kv_head = blockIdx.y;
-    const Block k = block_of(b, a, kQueries, blockIdx.x);
-    if (!k.exists) {
-        return;
-    }
-    const uint32_t runs = (k.chunks + plan.run - 1) / plan.run;
+__device__ __attribute__((always_inline)) inline void do_block(const Cache &c, const Batch &b, const Params &a,
+                                                               const Plan &plan, const Block &k, uint32_t kv_head,
+                                                               uint32_t from, uint32_t to, int place, uint32_t share,
+                                                               Shared<HD, QT> &sh, const T *q, T *out) {
+    constexpr uint32_t kQueries = 16 * QT;
     const uint32_t t = threadIdx.x;
-    if (run >= runs && !(run == 0 && k.chunks == 0)) {
-        return;
-    }
     const uint32_t wave = __builtin_amdgcn_readfirstlane(t / 64), lane = t % 64, n = lane % 16, g = lane / 16;
     const int32_t *const table = b.table + size_t(k.sequence) * b.stride;
-    const uint32_t end = k.first_chunk + min(k.chunks, (run + 1) * plan.run);
-    const uint32_t first = k.first_chunk + run * plan.run + wave;
+    const uint32_t end = k.first_chunk + min(k.chunks, to * kWaves);
+    const uint32_t first = k.first_chunk + from * kWaves + wave;
 
     Wave<HD, QT, kQueryPlanes<T>> w;
-    Places<TP> here{};
+    Places<TP> here{}, next{};
     Codes<HD> kc, vc;
+    // everything that the first chunk needs is requested before anything is waited for
     if (first < end) {
         here = places_of<TP>(c, table, first, k.lo, k.hi);
-        load_chunk<HD, TP>(c, kv_head, here, first, k.lo, k.hi, LaneOffsets<HD>(n, g), kc, vc);
+        next = places_of<TP>(c, table, min(first + kWaves, end - 1), k.lo, k.hi);
     }
+    RawQuery<HD, T> raw[QT];
 #pragma unroll
     for (int qi = 0; qi < QT; ++qi) {
         const uint32_t query = k.query0 + 16 * qi + n, token = k.rows == 1 ? 0u : query / a.group;
@@ -685,7 +723,7 @@ attention_split_kernel(Cache c, Batch b, Params a, Plan plan, const T *__restric
         w.mine[qi].first = a.window && position + 1 > int32_t(a.window) ? position + 1 - int32_t(a.window) : 0;
         const uint32_t row = k.row0 + (there ? token : 0u);
         const uint32_t head = kv_head * a.group + (there ? query - token * a.group : 0u);
-        load_query<HD, T>(q + (size_t(row) * a.heads + head) * HD, g, a.negate, w.qf[qi]);
+        raw[qi].load(q + (size_t(row) * a.heads + head) * HD, g);
         w.st.b[qi] = -INFINITY;
         w.st.l[qi] = 0.0f;
         w.nan_blocks[qi] = 0;
@@ -695,8 +733,16 @@ attention_split_kernel(Cache c, Batch b, Params a, Plan plan, const T *__restric
         }
     }
     if (first < end) {
+        load_chunk<HD, TP>(c, kv_head, here, first, k.lo, k.hi, LaneOffsets<HD>(n, g), kc, vc);
+    }
+#pragma unroll
+    for (int qi = 0; qi < QT; ++qi) {
+        raw[qi].planes(a.negate, w.qf[qi]);
+    }
+    if (first < end) {
         uint16_t *const lds = sh.v[wave];
-        const uint32_t at = walk<HD, T, QT, TP, false>(c, a, k, table, kv_head, first, end, kc, vc, here, lds, n, g, w);
+        const uint32_t at = walk<HD, T, QT, TP, false>(c, a, k, table, kv_head, first, end, kc, vc, here, next, lds, n, g,
+                                                       w);
         if (at < end) {
             Wave<HD, QT, kQueryPlanes<T>> copy = w;  // (the state itself stays in registers)
             walk_odd<HD, T, QT, TP>(c, a, k, table, kv_head, at, end, lds, n, g, copy);
@@ -729,37 +775,32 @@ attention_split_kernel(Cache c, Batch b, Params a, Plan plan, const T *__restric
         if (query >= k.rows * a.group) {
             break;
         }
-        const uint32_t token = query / a.group, row = k.row0 + token, head = kv_head * a.group + query % a.group;
-        T *const dst = out + (size_t(row) * a.heads + head) * HD + d;
-        if (k.bad || k.position0 + int32_t(token) < 0 || k.chunks == 0) {
-            if (run == 0) {
-                const float fill = k.bad ? __builtin_nanf("") : 0.0f;
-                store4(dst, f32x4{fill, fill, fill, fill});
-            }
-            continue;
-        }
         float top = sh.join.b[0][local];
 #pragma unroll
-        for (uint32_t w = 1; w < kWaves; ++w) {
-            top = fmaxf(top, sh.join.b[w][local]);
+        for (uint32_t x = 1; x < kWaves; ++x) {
+            top = fmaxf(top, sh.join.b[x][local]);
         }
         const float base = top == -INFINITY ? 0.0f : top;
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
         float l = 0.0f;
 #pragma unroll
-        for (uint32_t w = 0; w < kWaves; ++w) {
-            const float f = __builtin_amdgcn_exp2f(sh.join.b[w][local] - base);
-            const f32x4 x = *reinterpret_cast<const f32x4 *>(&sh.join.o[w][local][d]);
-            l = fmaf(sh.join.l[w][local], f, l);
+        for (uint32_t x = 0; x < kWaves; ++x) {
+            const float f = __builtin_amdgcn_exp2f(sh.join.b[x][local] - base);
+            const f32x4 y = *reinterpret_cast<const f32x4 *>(&sh.join.o[x][local][d]);
+            l = fmaf(sh.join.l[x][local], f, l);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                o[j] = fmaf(x[j], f, o[j]);
+                o[j] = fmaf(y[j], f, o[j]);
             }
         }
-        if (runs == 1) {
-            store4(dst, with_sink(a, head, top, o, l));
+        if (place < 0) {
+            const uint32_t token = k.rows == 1 ? 0u : query / a.group, row = k.row0 + token;
+            const uint32_t head = kv_head * a.group + query - token * a.group;
+            const bool idle = k.position0 + int32_t(token) < 0;
+            store4(out + (size_t(row) * a.heads + head) * HD + d,
+                   idle ? f32x4{0.f, 0.f, 0.f, 0.f} : with_sink(a, head, top, o, l));
         } else {
-            const size_t at = (size_t(run) * b.tokens + row) * a.heads + head;
+            const size_t at = ((size_t(kv_head) * plan.shares + share) * 2 + uint32_t(place)) * kQueries + local;
             *reinterpret_cast<f32x4 *>(plan.o + at * HD + d) = o;
             if (d == 0) {
                 plan.bl[at] = make_float2(top, l);
@@ -768,64 +809,195 @@ attention_split_kernel(Cache c, Batch b, Params a, Plan plan, const T *__restric
     }
 }
 
-// ---- the runs of a block joined: a wave per row and head -------------------------------------------
-
+// The outputs of a block whose rows see nothing: zeros, or NaN for a sequence that is too long.
 template <int HD, class T>
+__device__ inline void fill_block(const Params &a, uint32_t queries, const Block &k, uint32_t kv_head, T *out) {
+    for (uint32_t u = threadIdx.x; u < queries * (HD / 4); u += kThreads) {
+        const uint32_t query = k.query0 + u / (HD / 4), d = 4 * (u % (HD / 4));
+        if (query >= k.rows * a.group) {
+            break;
+        }
+        const uint32_t token = query / a.group, row = k.row0 + token, head = kv_head * a.group + query % a.group;
+        const float fill = k.bad && k.position0 + int32_t(token) >= 0 ? __builtin_nanf("") : 0.0f;
+        store4(out + (size_t(row) * a.heads + head) * HD + d, f32x4{fill, fill, fill, fill});
+    }
+}
+
+template <int HD, class T, int QT, int TP>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kResident<HD, T, QT>))) void
+attention_split_kernel(Cache c, Batch b, Params a, Plan plan, const T *__restrict__ q, T *__restrict__ out) {
+    constexpr uint32_t kQueries = 16 * QT;
+    __shared__ __attribute__((aligned(16))) Shared<HD, QT> sh;
+    const uint32_t share = blockIdx.x, kv_head = blockIdx.y, t = threadIdx.x;
+    uint32_t block = share, unit = 0, from = 0, to = 1;  // the block, its first unit, and the share's units
+    uint64_t total = 0;
+    uint32_t shares = 0;
+    if (!plan.single) {
+        // every workgroup sums up all blocks' units, and finds where its share begins
+        const uint32_t wave = t / 64, lane = t % 64;
+        const uint32_t per = (plan.blocks + kThreads - 1) / kThreads, first = t * per;
+        uint32_t mine = 0;
+        for (uint32_t i = first; i < min(first + per, plan.blocks); ++i) {
+            mine += block_of(b, a, kQueries, i).units();
+        }
+        uint32_t sum = mine;  // of the lanes up to this one
+#pragma unroll
+        for (uint32_t d = 1; d < 64; d <<= 1) {
+            const uint32_t x = __shfl_up(sum, d);
+            sum += lane >= d ? x : 0u;
+        }
+        if (lane == 63) {
+            sh.scan.sum[wave] = sum;
+        }
+        __syncthreads();
+        uint32_t before = sum - mine;
+#pragma unroll
+        for (uint32_t w = 0; w < kWaves; ++w) {
+            const uint32_t x = sh.scan.sum[w];
+            before += w < wave ? x : 0u;
+            total += x;
+        }
+        shares = uint32_t(min(uint64_t(plan.shares), total));  // a unit each at least
+        if (share >= shares) {
+            return;
+        }
+        from = uint32_t(total * share / shares);
+        to = uint32_t(total * (share + 1) / shares);
+        if (from >= before && from < before + mine) {
+            uint32_t at = before, i = first;
+            while (true) {
+                const uint32_t n = block_of(b, a, kQueries, i).units();
+                if (from < at + n) {
+                    break;
+                }
+                at += n;
+                ++i;
+            }
+            sh.scan.block = i;
+            sh.scan.first = at;
+        }
+        __syncthreads();
+        block = __builtin_amdgcn_readfirstlane(sh.scan.block);
+        unit = __builtin_amdgcn_readfirstlane(sh.scan.first);
+        __syncthreads();
+    }
+    while (unit < to) {
+        const Block k = block_of(b, a, kQueries, block);
+        const uint32_t units = k.units();
+        if (plan.single) {
+            if (units == 0) {
+                if (k.exists) {
+                    fill_block<HD, T>(a, kQueries, k, kv_head, out);
+                }
+                return;
+            }
+        }
+        if (units) {
+            const uint32_t x = max(from, unit), y = min(to, unit + units);
+            const int place = x == unit && y == unit + units ? -1 : x == unit ? 1 : 0;
+            if (place != 0 && !plan.single && kv_head == 0 && t == 0) {
+                // the share of a unit u is the last one that begins at u or before
+                const uint64_t last = (uint64_t(unit) + units) * shares - 1;
+                plan.span[block] = make_uint2(share, uint32_t(last / total));
+            }
+            do_block<HD, T, QT, TP>(c, b, a, plan, k, kv_head, x - unit, y - unit, place, share, sh, q, out);
+            __syncthreads();
+        }
+        unit += units;
+        ++block;
+    }
+}
+
+// ---- the parts of a block joined ---------------------------------------------------------------
+
+// W waves per row and head (4 where a block may have many parts, else 1): each takes a share of
+// the parts, 64 / (HD / 4) at a time.
+template <int HD, class T, int W>
 __global__ __launch_bounds__(kThreads) void attention_join_kernel(Cache c, Batch b, Params a, Plan plan,
                                                                   T *__restrict__ out) {
-    constexpr uint32_t kLanes = HD / 4, kParts = 64 / kLanes;  // lanes of an output, runs at a time
-    const uint32_t at = blockIdx.x * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const uint32_t row = at / a.heads, head = at % a.heads, lane = threadIdx.x % 64;
-    if (row >= b.tokens) {
-        return;
-    }
-    const kv4::Row r = kv4::row_of(b, row);
-    if (r.kind != kv4::kToken) {
-        return;
-    }
-    Block k{};
-    k.sequence = r.sequence;
-    k.row0 = b.starts ? uint32_t(max(b.starts[r.sequence], 0)) : r.sequence;
-    k.rows = b.starts ? min(uint32_t(max(b.starts[r.sequence + 1], 0)), b.tokens) - k.row0 : 1;
-    k.query0 = ((row - k.row0) * a.group + head % a.group) / plan.queries * plan.queries;
-    k = block_span(b, a, plan.queries, k);
-    const uint32_t runs = (k.chunks + plan.run - 1) / plan.run;
-    if (runs <= 1) {
-        return;
-    }
-    const size_t stride = size_t(b.tokens) * a.heads, base = size_t(row) * a.heads + head;
-    float top = -INFINITY;
-    for (uint32_t i = lane; i < runs; i += 64) {
-        top = fmaxf(top, plan.bl[i * stride + base].x);
-    }
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) {
-        top = fmaxf(top, __shfl_xor(top, d));
-    }
-    const float offset = top == -INFINITY ? 0.0f : top;
+    constexpr uint32_t kLanes = HD / 4, kParts = 64 / kLanes;  // lanes of an output, parts of a wave at a time
+    __shared__ float part_l[kWaves];
+    __shared__ f32x4 part_o[kWaves][kLanes];
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
+    const uint32_t at = blockIdx.x * (kWaves / W) + wave / W, turn = wave % W;
+    const uint32_t row = at / a.heads, head = at % a.heads, kv_head = head / a.group;
     const uint32_t part = lane / kLanes, d = 4 * (lane % kLanes);
-    f32x4 o = {0.f, 0.f, 0.f, 0.f};
-    float l = 0.0f;
-    for (uint32_t i = part; i < runs; i += kParts) {
-        const float2 s = plan.bl[i * stride + base];
-        const f32x4 x = *reinterpret_cast<const f32x4 *>(plan.o + (i * stride + base) * HD + d);
-        const float f = __builtin_amdgcn_exp2f(s.x - offset);
-        l = fmaf(s.y, f, l);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            o[j] = fmaf(x[j], f, o[j]);
+    T *const dst = out + (size_t(row) * a.heads + head) * HD + d;
+    uint32_t parts = 0, first = 0, local = 0;
+    if (row < b.tokens) {
+        const kv4::Row r = kv4::row_of(b, row);
+        if (r.kind == kv4::kToken) {
+            const uint32_t row0 = b.starts ? uint32_t(max(kv4::entry(b.starts, r.sequence), 0)) : r.sequence;
+            const uint32_t query = (row - row0) * a.group + head % a.group;
+            local = query % plan.queries;
+            const uint32_t block = b.starts ? uint32_t(uint64_t(row0) * a.group / plan.queries) + r.sequence
+                                            : r.sequence * ((a.group + plan.queries - 1) / plan.queries);
+            const uint2 span = plan.span[block + query / plan.queries];
+            first = span.x;
+            parts = span.y - span.x + 1;
+        } else if (r.kind != kv4::kPadding && turn == 0 && part == 0) {
+            const float fill = r.kind == kv4::kBad ? __builtin_nanf("") : 0.0f;
+            store4(dst, f32x4{fill, fill, fill, fill});
         }
     }
+    if (W == 1 && parts <= 1) {
+        return;  // (one part: the workgroup that had it wrote the output)
+    }
+    const auto place = [&](uint32_t i) {
+        return ((size_t(kv_head) * plan.shares + first + i) * 2 + (i == 0 ? 1 : 0)) * plan.queries + local;
+    };
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    float top = -INFINITY, l = 0.0f;
+    if (parts > 1) {
+        for (uint32_t i = lane; i < parts; i += 64) {
+            top = fmaxf(top, plan.bl[place(i)].x);
+        }
 #pragma unroll
-    for (uint32_t x = kLanes; x < 64; x <<= 1) {
-        l += __shfl_xor(l, x);
+        for (int x = 32; x >= 1; x >>= 1) {
+            top = fmaxf(top, __shfl_xor(top, x));
+        }
+        const float offset = top == -INFINITY ? 0.0f : top;
+#pragma unroll 4
+        for (uint32_t i = turn * kParts + part; i < parts; i += W * kParts) {
+            const float2 s = plan.bl[place(i)];
+            const f32x4 x = *reinterpret_cast<const f32x4 *>(plan.o + place(i) * HD + d);
+            const float f = __builtin_amdgcn_exp2f(s.x - offset);
+            l = fmaf(s.y, f, l);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            o[j] += __shfl_xor(o[j], x);
+            for (int j = 0; j < 4; ++j) {
+                o[j] = fmaf(x[j], f, o[j]);
+            }
+        }
+#pragma unroll
+        for (uint32_t x = kLanes; x < 64; x <<= 1) {
+            l += __shfl_xor(l, x);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                o[j] += __shfl_xor(o[j], x);
+            }
+        }
+    }
+    if (W > 1) {
+        if (part == 0) {
+            part_o[wave][lane] = o;
+            part_l[wave] = l;
+        }
+        __syncthreads();
+        if (turn != 0 || parts <= 1) {
+            return;
+        }
+#pragma unroll
+        for (uint32_t x = 1; x < W; ++x) {
+            l += part_l[wave + x];
+            const f32x4 y = part_o[wave + x][lane % kLanes];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                o[j] += y[j];
+            }
         }
     }
     if (part == 0) {
-        store4(out + base * HD + d, with_sink(a, head, top, o, l));
+        store4(dst, with_sink(a, head, top, o, l));
     }
 }
 
@@ -847,17 +1019,25 @@ int check_attention(const ttl_kv4_cache *cache, const ttl_kv4_batch *batch, cons
     return TTL_OK;
 }
 
-constexpr uint32_t kMaxSplits = 256;
+uint32_t resident_groups(uint32_t head_dim, int dtype, uint32_t tiles) {
+    const bool f32 = dtype == TTL_DTYPE_F32;
+    if (head_dim == 64) {
+        return tiles == 2 ? (f32 ? kResident<64, float, 2> : kResident<64, __bf16, 2>)
+                          : (f32 ? kResident<64, float, 1> : kResident<64, __bf16, 1>);
+    }
+    return tiles == 2 ? (f32 ? kResident<128, float, 2> : kResident<128, __bf16, 2>)
+                      : (f32 ? kResident<128, float, 1> : kResident<128, __bf16, 1>);
+}
 
-// The cut of a checked call: query tiles per wave by the queries a sequence has on average;
-// runs of chunks so that about kTargetGroups workgroups share the longest sequence's walk.
+// The cut of a checked call: query tiles of a wave by the queries a sequence has on average, a
+// share for every workgroup that the card's 256 CUs hold at once.
 struct Cut {
     uint32_t tiles;
     Plan plan;
+    uint32_t most_parts;  // of a block
     size_t workspace;
 };
 Cut cut_of(const ttl_kv4_cache *cache, const ttl_kv4_batch *batch, const ttl_kv4_attention *attention) {
-    constexpr uint64_t kTargetGroups = 2048;
     const uint32_t group = attention->heads / cache->kv_heads;
     Cut cut{};
     const uint64_t queries = uint64_t(batch->tokens) * group;  // of a key/value head
@@ -873,16 +1053,19 @@ Cut cut_of(const ttl_kv4_cache *cache, const ttl_kv4_batch *batch, const ttl_kv4
         longest = uint32_t(std::min<uint64_t>(longest, uint64_t(attention->window) + p.queries / group + 1));
     }
     const uint32_t chunks = longest / kChunk + (attention->window ? 2 : 1);  // any alignment
-    const uint64_t groups = uint64_t(p.blocks) * cache->kv_heads;
-    const uint64_t splits =
-        std::max<uint64_t>(1, std::min<uint64_t>({kTargetGroups / groups, chunks / kWaves, kMaxSplits}));
-    p.run = uint32_t((chunks + splits - 1) / splits);
-    p.run = (p.run + kWaves - 1) / kWaves * kWaves;
-    p.splits = (chunks + p.run - 1) / p.run;
-    if (p.splits > 1) {
-        const size_t rows = size_t(p.splits) * batch->tokens * attention->heads;
-        cut.workspace = rows * (cache->head_dim * sizeof(float) + sizeof(float2));
+    const uint64_t units = (chunks + kWaves - 1) / kWaves;
+    p.single = units == 1;
+    if (p.single) {
+        p.shares = p.blocks;
+        return cut;
     }
+    const uint32_t resident = resident_groups(cache->head_dim, attention->dtype, cut.tiles);
+    p.shares = std::max(1u, 256 * resident / cache->kv_heads);
+    p.shares = uint32_t(std::min<uint64_t>(p.shares, units * p.blocks));
+    // a block spans the shares of its units
+    cut.most_parts = uint32_t(std::min<uint64_t>(p.shares, units + 1));
+    const size_t places = size_t(cache->kv_heads) * p.shares * 2 * p.queries;
+    cut.workspace = places * (cache->head_dim * sizeof(float) + sizeof(float2)) + size_t(p.blocks) * sizeof(uint2);
     return cut;
 }
 
@@ -906,7 +1089,7 @@ int run_attention(ttl_ctx *ctx, const ttl_kv4_cache *cache, const ttl_kv4_batch 
                 cut.workspace);
     TTL_REQUIRE(cut.workspace == 0 || (uintptr_t(workspace) & 255) == 0, TTL_ERR_INVALID,
                 "%s: the workspace must be 256-byte aligned", what);
-    const uint64_t groups = uint64_t(cut.plan.blocks) * cache->kv_heads * cut.plan.splits;
+    const uint64_t groups = uint64_t(cut.plan.shares) * cache->kv_heads;
     TTL_REQUIRE(groups * kThreads <= 0xffffffffu && uint64_t(batch->tokens) * attention->heads <= 0x7fffffffu, TTL_ERR_SHAPE,
                 "%s: %u tokens of %u heads are too many for one call", what, batch->tokens, attention->heads);
     TTL_HIP(hipSetDevice(ctx->device));
@@ -923,16 +1106,18 @@ int run_attention(ttl_ctx *ctx, const ttl_kv4_cache *cache, const ttl_kv4_batch 
     a.c_lo = scale > 0x1p-120 ? float((scale - double(a.c)) / double(a.c)) : 0.0f;
     a.negate = attention->scale < 0.0f;
     Plan p = cut.plan;
-    if (p.splits > 1) {
+    if (!p.single) {
+        const size_t places = size_t(cache->kv_heads) * p.shares * 2 * p.queries;
         p.o = static_cast<float *>(workspace);
-        p.bl = reinterpret_cast<float2 *>(p.o + size_t(p.splits) * b.tokens * a.heads * cache->head_dim);
+        p.bl = reinterpret_cast<float2 *>(p.o + places * cache->head_dim);
+        p.span = reinterpret_cast<uint2 *>(p.bl + places);
     }
     const auto launch = [&](auto hd, auto zero) {
         constexpr int HD = decltype(hd)::value;
         using T = decltype(zero);
         const T *qt = static_cast<const T *>(q);
         T *ot = static_cast<T *>(out);
-        const dim3 grid(p.blocks, c.kv_heads, p.splits);
+        const dim3 grid(p.shares, c.kv_heads);
         const bool big = c.page_shift >= 6;
         const auto split = [&](auto tiles) {
             constexpr int QT = decltype(tiles)::value;
@@ -947,9 +1132,14 @@ int run_attention(ttl_ctx *ctx, const ttl_kv4_cache *cache, const ttl_kv4_batch 
         } else {
             split(std::integral_constant<int, 2>());
         }
-        if (p.splits > 1) {
-            attention_join_kernel<HD, T><<<ttl::blocks_for(size_t(b.tokens) * a.heads, kWaves), kThreads, 0,
-                                           ctx->stream>>>(c, b, a, p, ot);
+        if (!p.single) {
+            const size_t rows = size_t(b.tokens) * a.heads;
+            if (cut.most_parts > 16 && rows <= 4096) {
+                attention_join_kernel<HD, T, 4><<<uint32_t(rows), kThreads, 0, ctx->stream>>>(c, b, a, p, ot);
+            } else {
+                attention_join_kernel<HD, T, 1><<<ttl::blocks_for(rows, kWaves), kThreads, 0, ctx->stream>>>(c, b, a, p,
+                                                                                                     ot);
+            }
         }
     };
     if (cache->head_dim == 64) {
