@@ -50,6 +50,18 @@ constexpr float kLog2e = 0x1.715476p+0f, kLog2eLo = 0x1.4ae0cp-26f;  // log2 e =
 constexpr uint32_t kF16First = 104, kF16Last = 140;                  // scale bytes of V on the f16 path
 constexpr float kWeightShift = 11.0f;                               // weights are held times 2^11
 
+// How a wave's 16 columns are used (M): kHalf for 8 queries or fewer, columns 8..15 the same
+// queries on the other half of the chunk (so that no lane weighs scores that nobody asked for);
+// kOne and kTwo for 16 queries, and 32 in two column tiles.
+constexpr int kHalf = 0, kOne = 1, kTwo = 2;
+template <int M>
+struct Mode {
+    static constexpr int columns = M == kTwo ? 2 : 1;             // column tiles
+    static constexpr int halves = M == kHalf ? 2 : 1;
+    static constexpr int tiles = 4 / halves;                      // position tiles of a lane's column
+    static constexpr uint32_t queries = M == kHalf ? 8 : 16 * columns;
+};
+
 struct Params {
     const float *sinks;
     uint32_t heads, group, window;
@@ -193,34 +205,30 @@ struct LaneOffsets {
         : code(n * Layout<HD>::code_bytes + g * (HD / 8)), scale(n * Layout<HD>::scale_bytes + g * (HD / 4) / 32) {}
 };
 
-template <int HD, int TP>
-__device__ __attribute__((always_inline)) inline void load_chunk(const Cache &c, uint32_t kv_head,
+// The codes and scales of a chunk's K or V.
+template <int HD, int TP, bool V>
+__device__ __attribute__((always_inline)) inline void load_codes(const Cache &c, const uint8_t *head, size_t page_bytes,
                                                                  const Places<TP> &places, uint32_t chunk, uint32_t lo,
-                                                                 uint32_t hi, const LaneOffsets<HD> &at, Codes<HD> &k,
-                                                                 Codes<HD> &v) {
+                                                                 uint32_t hi, const LaneOffsets<HD> &at, Codes<HD> &x) {
     using L = Layout<HD>;
     const uint32_t mask = (1u << c.page_shift) - 1;
-    const uint8_t *kp = nullptr, *vp = nullptr, *ks = nullptr, *vs = nullptr;  // uniform
+    const uint8_t *codes = nullptr, *scales = nullptr;  // uniform
 #pragma unroll
     for (uint32_t i = 0; i < kTiles; ++i) {
         if (TP != 1 || i == 0) {
             const uint32_t tile = TP == 1 ? chunk * kTiles : min(max(chunk * kTiles + i, lo / 16), hi / 16);
             const uint32_t page = places.page[i], slot = (tile * 16) & mask;
-            const uint8_t *rec = kv4::record_of(c, page < c.pages ? page : 0u, kv_head);
-            kp = rec + L::k_codes(slot);
-            vp = rec + L::v_codes(c.page_shift, slot);
-            ks = rec + L::k_scales(c.page_shift, slot);
-            vs = rec + L::v_scales(c.page_shift, slot);
+            const uint8_t *rec = head + (page < c.pages ? page : 0u) * page_bytes;
+            codes = rec + (V ? L::v_codes(c.page_shift, slot) : L::k_codes(slot));
+            scales = rec + (V ? L::v_scales(c.page_shift, slot) : L::k_scales(c.page_shift, slot));
         }
         const uint32_t tile_code = TP == 1 ? i * 16 * L::code_bytes : 0, tile_scale = TP == 1 ? i * 16 * L::scale_bytes : 0;
-        load_words<HD>(kp + (at.code + tile_code), k.w[i]);
-        load_words<HD>(vp + (at.code + tile_code), v.w[i]);
-        k.scale[i] = ks[at.scale + tile_scale];
-        v.scale[i] = vs[at.scale + tile_scale];
+        load_words<HD>(codes + (at.code + tile_code), x.w[i]);
+        x.scale[i] = scales[at.scale + tile_scale];
     }
 }
 
-// What load_chunk left to do for chunks at an end of lo..hi or of the pool: keys of a page
+// What load_codes left to do for chunks at an end of lo..hi or of the pool: keys of a page
 // that is not there read as NaN, values outside lo..hi as zeros.
 template <int HD, int TP>
 __device__ __attribute__((always_inline)) inline void trim_chunk(const Cache &c, const Places<TP> &places,
@@ -254,11 +262,11 @@ __device__ __attribute__((always_inline)) inline bool all_in_pool(const Cache &c
 
 // ---- the running softmax of a wave's queries ----------------------------------------------------
 
-template <int HD, int QT>
+template <int HD, int M>
 struct State {
-    float b[QT];  // offset: c x a large score - 11; weights are 2^(c s - b), 2^15 at most
-    float l[QT];  // the lane's share of their sum
-    f32x4 o[QT][HD / 16];  // O^T: dims 16 mt + 4g + i of column n
+    float b[Mode<M>::columns];  // offset: c x a large score - 11; weights are 2^(c s - b), 2^15 at most
+    float l[Mode<M>::columns];  // the lane's share of their sum
+    f32x4 o[Mode<M>::columns][HD / 16];  // O^T: dims 16 mt + 4g + i of column n
 };
 
 __device__ inline float max_over_groups(float x) {
@@ -286,40 +294,41 @@ struct Query {
 };
 
 // Scores to weights.  The offset follows the largest score lazily: it is set anew (and what is
-// there rescaled) only when a lane's 16 weights pass 2^15 together, before which none leaves
+// there rescaled) only when a lane's weights pass 2^15 together, before which none leaves
 // the f16 range, or before any score was seen (its weights are then infinite).
-template <int HD, int QT>
-__device__ __attribute__((always_inline)) inline void softmax_step(f32x4 (&s)[kTiles], State<HD, QT> &st, int qi,
-                                                                   const Query &q, bool whole, uint32_t chunk,
-                                                                   uint32_t g, float c) {
+// `at`: the position of the lane's first score.
+template <int HD, int M>
+__device__ __attribute__((always_inline)) inline void softmax_step(f32x4 (&s)[Mode<M>::tiles], State<HD, M> &st, int qi,
+                                                                   const Query &q, bool whole, int32_t at, float c) {
+    constexpr int NT = Mode<M>::tiles;
     if (!whole) {
 #pragma unroll
-        for (uint32_t i = 0; i < kTiles; ++i) {
+        for (int i = 0; i < NT; ++i) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int32_t at = int32_t(chunk * kChunk + 16 * i + 4 * g) + j;
-                s[i][j] = at >= q.first && at <= q.last ? s[i][j] : -INFINITY;
+                const int32_t p = at + 16 * i + j;
+                s[i][j] = p >= q.first && p <= q.last ? s[i][j] : -INFINITY;
             }
         }
     }
-    const auto weigh = [&](float base, f32x4 (&p)[kTiles]) __attribute__((always_inline)) {
-        float sum = 0.0f;
+    const auto weigh = [&](float base, f32x4 (&p)[NT]) __attribute__((always_inline)) {
+        f32x4 sum;
 #pragma unroll
-        for (uint32_t i = 0; i < kTiles; ++i) {
+        for (int i = 0; i < NT; ++i) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 p[i][j] = __builtin_amdgcn_exp2f(fmaf(s[i][j], c, -base));
-                sum += p[i][j];
+                sum[j] = i ? sum[j] + p[i][j] : p[i][j];
             }
         }
-        return sum;
+        return (sum[0] + sum[1]) + (sum[2] + sum[3]);
     };
-    f32x4 p[kTiles];
+    f32x4 p[NT];
     float sum = weigh(st.b[qi], p);
     if (__any(!(sum <= 0x1p15f))) {
         float m = s[0][0];
 #pragma unroll
-        for (uint32_t i = 0; i < kTiles; ++i) {
+        for (int i = 0; i < NT; ++i) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 m = fmaxf(m, s[i][j]);
@@ -342,7 +351,7 @@ __device__ __attribute__((always_inline)) inline void softmax_step(f32x4 (&s)[kT
     }
     st.l[qi] += sum;
 #pragma unroll
-    for (uint32_t i = 0; i < kTiles; ++i) {
+    for (int i = 0; i < NT; ++i) {
         s[i] = p[i];
     }
 }
@@ -412,18 +421,66 @@ __device__ __attribute__((always_inline)) inline V value_fragment(const uint16_t
     return __builtin_bit_cast(V, s16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
 }
 
-template <int HD, class V, int PP, int QT>
-__device__ __attribute__((always_inline)) inline void weigh_values(const uint16_t *lds, const f32x4 (&s)[QT][kTiles],
-                                                                   State<HD, QT> &st, uint32_t n, uint32_t g) {
-    constexpr int kSteps = int(kTiles) / 2, kBatch = 4;  // fragments requested together, a batch ahead
+// The weights' planes left in s, one at a time (and few registers) for the bf16 path.
+template <int HD, int M>
+__device__ __attribute__((always_inline)) inline void weigh_values_odd(
+    const uint16_t *lds, f32x4 (&s)[Mode<M>::columns][Mode<M>::tiles], State<HD, M> &st, uint32_t n, uint32_t g) {
+    constexpr int QT = Mode<M>::columns, NT = Mode<M>::tiles;
+#pragma unroll 1
+    for (int plane = 0; plane < 3; ++plane) {
+#pragma unroll
+        for (int h = 0; h < int(kTiles) / 2; ++h) {
+            bf16x8 p[QT];
+#pragma unroll
+            for (int qi = 0; qi < QT; ++qi) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int i = (M == kHalf ? 0 : 2 * h) + j / 4;
+                    const __bf16 x = __bf16(s[qi][i][j % 4]);
+                    p[qi][j] = M != kHalf || int(n / 8) == h ? x : __bf16(0.0f);
+                }
+            }
+#pragma unroll
+            for (int mt = 0; mt < HD / 16; ++mt) {
+                const bf16x8 a = value_fragment<HD, bf16x8>(lds, h, mt, n, g);
+#pragma unroll
+                for (int qi = 0; qi < QT; ++qi) {
+                    st.o[qi][mt] = mf::mfma(a, p[qi], st.o[qi][mt]);
+                }
+            }
+        }
+#pragma unroll
+        for (int qi = 0; qi < QT; ++qi) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    s[qi][i][j] -= float(__bf16(s[qi][i][j]));
+                }
+            }
+        }
+    }
+}
+
+template <int HD, class V, int PP, int M>
+__device__ __attribute__((always_inline)) inline void weigh_values(
+    const uint16_t *lds, const f32x4 (&s)[Mode<M>::columns][Mode<M>::tiles], State<HD, M> &st, uint32_t n, uint32_t g) {
+    constexpr int QT = Mode<M>::columns;
+    // fragments requested together, and a batch ahead where the registers are there
+    constexpr int kSteps = int(kTiles) / 2, kBatch = 4, kBuffers = PP == 2 ? 2 : 1;
     constexpr int kFragments = kSteps * (HD / 16);
     const auto fragment = [&](int f) __attribute__((always_inline)) {
         return value_fragment<HD, V>(lds, f / (HD / 16), f % (HD / 16), n, g);
     };
-    V a[2][kBatch];
+    V a[kBuffers][kBatch];
+    const auto request = [&](int f0) __attribute__((always_inline)) {
 #pragma unroll
-    for (int f = 0; f < kBatch; ++f) {
-        a[0][f] = fragment(f);
+        for (int f = 0; f < kBatch; ++f) {
+            a[f0 / kBatch % kBuffers][f] = fragment(f0 + f);
+        }
+    };
+    if (kBuffers == 2) {
+        request(0);
     }
     V p[QT][PP];
 #pragma unroll
@@ -432,20 +489,26 @@ __device__ __attribute__((always_inline)) inline void weigh_values(const uint16_
         if (f0 % (HD / 16) == 0) {
 #pragma unroll
             for (int qi = 0; qi < QT; ++qi) {
+                constexpr int kOwn = M == kHalf ? 0 : 2;
                 float x[8];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    x[j] = s[qi][2 * h][j];
-                    x[4 + j] = s[qi][2 * h + 1][j];
+                    x[j] = s[qi][kOwn * h][j];
+                    x[4 + j] = s[qi][kOwn * h + 1][j];
                 }
                 split<V, PP>(x, p[qi]);
+                if (M == kHalf) {  // the lane's tiles are K step 0 in columns 0..7, step 1 in 8..15
+#pragma unroll
+                    for (int k = 0; k < PP; ++k) {
+                        const mf::u32x4 w = __builtin_bit_cast(mf::u32x4, p[qi][k]);
+                        p[qi][k] = __builtin_bit_cast(V, int(n / 8) == h ? w : mf::u32x4{0u, 0u, 0u, 0u});
+                    }
+                }
             }
         }
-        if (f0 + kBatch < kFragments) {
-#pragma unroll
-            for (int f = 0; f < kBatch; ++f) {
-                a[(f0 / kBatch + 1) % 2][f] = fragment(f0 + kBatch + f);
-            }
+        const int ahead = f0 + (kBuffers - 1) * kBatch;
+        if (ahead < kFragments) {
+            request(ahead);
         }
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -455,7 +518,7 @@ __device__ __attribute__((always_inline)) inline void weigh_values(const uint16_
                 const int mt = (f0 + f) % (HD / 16);
 #pragma unroll
                 for (int qi = 0; qi < QT; ++qi) {
-                    st.o[qi][mt] = mf::mfma(a[f0 / kBatch % 2][f], p[qi][k], st.o[qi][mt]);
+                    st.o[qi][mt] = mf::mfma(a[f0 / kBatch % kBuffers][f], p[qi][k], st.o[qi][mt]);
                 }
             }
         }
@@ -537,36 +600,50 @@ __device__ inline f32x4 with_sink(const Params &a, uint32_t head, float b, f32x4
 
 // ---- few queries: the waves of a workgroup share them and take the chunks in turn -----------------
 
-template <int HD, int QT, int QP>
+template <int HD, int M, int QP>
 struct Wave {
-    State<HD, QT> st;
-    bf16x8 qf[QT][HD / 32][QP];
-    Query mine[QT];
-    uint32_t nan_blocks[QT];  // blocks of V (a bit each) that hold a NaN the query sees, by lane
+    State<HD, M> st;
+    bf16x8 qf[Mode<M>::columns][HD / 32][QP];
+    Query mine[Mode<M>::columns];
+    uint32_t nan_blocks[Mode<M>::columns];  // blocks of V (a bit each) with a NaN that the query sees, by lane
 };
 
-// A wave's chunks from `chunk` on, every kWaves-th below `end`.  ODD false: it returns at the
-// first chunk with a scale byte of V outside the f16 path's (its number, or one past the
-// end); ODD true: it takes every chunk to the end on the bf16 path.  A loop of its own for each
-// keeps the running state in registers.
-template <int HD, class T, int QT, int TP, bool ODD>
-__device__ __attribute__((always_inline)) inline uint32_t walk(const Cache &c, const Params &a, const Block &k,
-                                                               const int32_t *table, uint32_t kv_head, uint32_t chunk,
-                                                               uint32_t end, Codes<HD> &kc, Codes<HD> &vc,
-                                                               Places<TP> here, Places<TP> next, uint16_t *lds,
-                                                               uint32_t n, uint32_t g,
-                                                               Wave<HD, QT, kQueryPlanes<T>> &w) {
-    constexpr int NS = HD / 32, QP = kQueryPlanes<T>, PP = kWeightPlanes<T>;
-    const LaneOffsets<HD> at(n, g);
+// Where a block's chunks come from.
+template <int TP>
+struct Source {
+    const int32_t *table;
+    const uint8_t *head;  // the key/value head's record of page 0
+    size_t page_bytes;
+    uint32_t lo, hi;
     // the smallest last and the largest first position of the block's queries, for whole chunks
-    const uint32_t last_min = uint32_t(max(k.position0 + int32_t(k.query0 / a.group), 0));
-    const uint32_t first_max = a.window && k.hi + 1 > a.window ? k.hi + 1 - a.window : 0;
+    uint32_t last_min, first_max;
+    __device__ Places<TP> places(const Cache &c, uint32_t chunk) const {
+        return places_of<TP>(c, table, chunk, lo, hi);
+    }
+};
+
+// A wave's chunks from `chunk` on, every kWaves-th below `end`; kc and vc hold the first one's
+// codes.  ODD false: it returns at the first chunk with a scale byte of V outside the f16
+// path's (its number, or one past the end); ODD true: it takes every chunk to the end on the
+// bf16 path.  A loop of its own for each keeps the running state in registers.  The next
+// chunk's K is requested when this one's is multiplied, its V when this one's is in LDS, into
+// the same registers.
+template <int HD, class T, int M, int TP, bool ODD>
+__device__ __attribute__((always_inline)) inline uint32_t walk(const Cache &c, const Params &a, const Source<TP> &src,
+                                                               uint32_t chunk, uint32_t end, Codes<HD> &kc,
+                                                               Codes<HD> &vc, Places<TP> here, Places<TP> next,
+                                                               uint16_t *lds, uint32_t n, uint32_t g,
+                                                               Wave<HD, M, kQueryPlanes<T>> &w) {
+    constexpr int NS = HD / 32, QP = kQueryPlanes<T>, PP = kWeightPlanes<T>, QT = Mode<M>::columns;
+    constexpr int NT = Mode<M>::tiles;
+    const LaneOffsets<HD> at(n, g);
+    const bool upper = M == kHalf && n >= 8;
     while (true) {
         const uint32_t c0 = chunk * kChunk;
-        const bool inside = c0 >= k.lo && c0 + kChunk - 1 <= k.hi;
-        const bool whole = c0 >= first_max && c0 + kChunk - 1 <= last_min;
+        const bool inside = c0 >= src.lo && c0 + kChunk - 1 <= src.hi;
+        const bool whole = c0 >= src.first_max && c0 + kChunk - 1 <= src.last_min;
         if (!inside || !all_in_pool(c, here)) {
-            trim_chunk<HD, TP>(c, here, chunk, k.lo, k.hi, n, kc, vc);
+            trim_chunk<HD, TP>(c, here, chunk, src.lo, src.hi, n, kc, vc);
         }
         if (!ODD) {
             uint32_t far = 0;
@@ -579,29 +656,32 @@ __device__ __attribute__((always_inline)) inline uint32_t walk(const Cache &c, c
             }
         }
         const uint32_t ahead = min(chunk + kWaves, end - 1);
-        Codes<HD> kn, vn;
         here = next;
-        next = places_of<TP>(c, table, min(chunk + 2 * kWaves, end - 1), k.lo, k.hi);
-        load_chunk<HD, TP>(c, kv_head, here, ahead, k.lo, k.hi, at, kn, vn);
+        next = src.places(c, min(chunk + 2 * kWaves, end - 1));
 
-        // S^T
-        f32x4 s[QT][kTiles];
+        // S^T, the tiles side by side: products of one accumulator wait for each other
+        f32x4 st[QT][kTiles];
 #pragma unroll
-        for (uint32_t i = 0; i < kTiles; ++i) {
-            const float scale = kv4::scale_of(kc.scale[i]);
+        for (int ks = 0; ks < NS; ++ks) {
+            bf16x8 kf[kTiles];
 #pragma unroll
-            for (int ks = 0; ks < NS; ++ks) {
-                const bf16x8 kf = mf::decode_step(kc.w[i][ks], scale);
+            for (uint32_t i = 0; i < kTiles; ++i) {
+                kf[i] = mf::decode_step(kc.w[i][ks], kv4::scale_of(kc.scale[i]));
+            }
 #pragma unroll
-                for (int p = QP - 1; p >= 0; --p) {
+            for (int p = QP - 1; p >= 0; --p) {
+#pragma unroll
+                for (uint32_t i = 0; i < kTiles; ++i) {
 #pragma unroll
                     for (int qi = 0; qi < QT; ++qi) {
-                        s[qi][i] = mf::mfma(kf, w.qf[qi][ks][p],
-                                            ks == 0 && p == QP - 1 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[qi][i]);
+                        st[qi][i] = mf::mfma(kf[i], w.qf[qi][ks][p],
+                                             ks == 0 && p == QP - 1 ? f32x4{0.f, 0.f, 0.f, 0.f} : st[qi][i]);
                     }
                 }
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
+        load_codes<HD, TP, false>(c, src.head, src.page_bytes, here, ahead, src.lo, src.hi, at, kc);
         if (ODD) {
             // NaN blocks of a position, a bit each, behind its row (its lanes are n, n + 16,
             // n + 32, n + 48); their values are zeros here
@@ -622,20 +702,32 @@ __device__ __attribute__((always_inline)) inline uint32_t walk(const Cache &c, c
         } else {
             stage_values<HD, f16x8>(lds, vc, n, g);
         }
+        __builtin_amdgcn_sched_barrier(0);
+        load_codes<HD, TP, true>(c, src.head, src.page_bytes, here, ahead, src.lo, src.hi, at, vc);
+
+        f32x4 s[QT][NT];
+        const int32_t at0 = int32_t(c0 + 4 * g) + (upper ? 32 : 0);
 #pragma unroll
         for (int qi = 0; qi < QT; ++qi) {
-            softmax_step<HD, QT>(s[qi], w.st, qi, w.mine[qi], whole, chunk, g, a.c);
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    s[qi][i][j] = M == kHalf && upper ? st[qi][i + kTiles - NT][j] : st[qi][i][j];
+                }
+            }
+            softmax_step<HD, M>(s[qi], w.st, qi, w.mine[qi], whole, at0, a.c);
         }
         __builtin_amdgcn_wave_barrier();
         asm volatile("" ::: "memory");
         if (ODD) {
-            weigh_values<HD, bf16x8, 3, QT>(lds, s, w.st, n, g);
+            weigh_values_odd<HD, M>(lds, s, w.st, n, g);
 #pragma unroll
-            for (uint32_t i = 0; i < kTiles; ++i) {
+            for (int i = 0; i < NT; ++i) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const uint32_t bits = lds[(16 * i + 4 * g + j) * kVStride<HD> + HD];
-                    const int32_t p = int32_t(c0 + 16 * i + 4 * g) + j;
+                    const int32_t p = at0 + 16 * i + j;
+                    const uint32_t bits = lds[(p - int32_t(c0)) * int32_t(kVStride<HD>) + HD];
 #pragma unroll
                     for (int qi = 0; qi < QT; ++qi) {
                         w.nan_blocks[qi] |= p >= w.mine[qi].first && p <= w.mine[qi].last ? bits : 0u;
@@ -643,7 +735,7 @@ __device__ __attribute__((always_inline)) inline uint32_t walk(const Cache &c, c
                 }
             }
         } else {
-            weigh_values<HD, f16x8, PP, QT>(lds, s, w.st, n, g);
+            weigh_values<HD, f16x8, PP, M>(lds, s, w.st, n, g);
         }
         asm volatile("" ::: "memory");
         __builtin_amdgcn_wave_barrier();
@@ -651,39 +743,34 @@ __device__ __attribute__((always_inline)) inline uint32_t walk(const Cache &c, c
         if (chunk >= end) {
             return chunk;
         }
-        kc = kn;
-        vc = vn;
     }
 }
 
-// The walk on the bf16 path, with a copy of the state, so that the other walk's stays in
-// registers of its own.
-template <int HD, class T, int QT, int TP>
-__device__ __attribute__((always_inline)) inline void walk_odd(const Cache &c, const Params &a, const Block &k,
-                                                   const int32_t *table, uint32_t kv_head, uint32_t chunk,
-                                                   uint32_t end, uint16_t *lds, uint32_t n, uint32_t g,
-                                                   Wave<HD, QT, kQueryPlanes<T>> &w) {
-    const Places<TP> here = places_of<TP>(c, table, chunk, k.lo, k.hi);
+// The walk on the bf16 path, which requests its first chunk again.
+template <int HD, class T, int M, int TP>
+__device__ __attribute__((always_inline)) inline void walk_odd(const Cache &c, const Params &a, const Source<TP> &src,
+                                                               uint32_t chunk, uint32_t end, uint16_t *lds, uint32_t n,
+                                                               uint32_t g, Wave<HD, M, kQueryPlanes<T>> &w) {
+    const Places<TP> here = src.places(c, chunk), next = src.places(c, min(chunk + kWaves, end - 1));
     Codes<HD> kc, vc;
-    load_chunk<HD, TP>(c, kv_head, here, chunk, k.lo, k.hi, LaneOffsets<HD>(n, g), kc, vc);
-    Wave<HD, QT, kQueryPlanes<T>> mine = w;
-    const Places<TP> next = places_of<TP>(c, table, min(chunk + kWaves, end - 1), k.lo, k.hi);
-    walk<HD, T, QT, TP, true>(c, a, k, table, kv_head, chunk, end, kc, vc, here, next, lds, n, g, mine);
-    w = mine;
+    load_codes<HD, TP, false>(c, src.head, src.page_bytes, here, chunk, src.lo, src.hi, LaneOffsets<HD>(n, g), kc);
+    load_codes<HD, TP, true>(c, src.head, src.page_bytes, here, chunk, src.lo, src.hi, LaneOffsets<HD>(n, g), vc);
+    walk<HD, T, M, TP, true>(c, a, src, chunk, end, kc, vc, here, next, lds, n, g, w);
 }
 
-// What bounds it: at long contexts the cache's bytes.  (Figures with the launch.)
-// Waves per SIMD that the kernel's registers leave room for.
-template <int HD, class T, int QT>
-constexpr int kResident = QT == 2 ? (HD == 64 ? 2 : 1) : HD == 128 ? 2 : 3;
+// Workgroups of a CU (waves of a SIMD).  More would fit on 128 registers with M kHalf, and were
+// slower: 4 instead of 3 for bf16 queries 51.8 against 49.8 us (64 ragged sequences up to
+// 8192), 3 instead of 2 for f32 79.9 against 74.1 us (128 at 4096).
+template <int HD, class T, int M>
+constexpr int kResident = M == kTwo ? (HD == 64 ? 2 : 1) : HD == 128 || std::is_same<T, float>::value ? 2 : 3;
 
-template <int HD, int QT>
+template <int HD, int M>
 union Shared {
     static constexpr uint32_t kOStride = HD + 4;
     uint16_t v[kWaves][kChunk * kVStride<HD>];
     struct {
-        float o[kWaves][16 * QT][kOStride];
-        float b[kWaves][16 * QT], l[kWaves][16 * QT];
+        float o[kWaves][16 * Mode<M>::columns][kOStride];
+        float b[kWaves][16 * Mode<M>::columns], l[kWaves][16 * Mode<M>::columns];
     } join;
     struct {
         uint32_t sum[kWaves];
@@ -693,30 +780,42 @@ union Shared {
 
 // Units [from, to) of a block: the waves take its chunks in turn, and their states are joined.
 // place < 0: the block is whole, its outputs are written; else the place of the share's part.
-template <int HD, class T, int QT, int TP>
+template <int HD, class T, int M, int TP>
 __device__ __attribute__((always_inline)) inline void do_block(const Cache &c, const Batch &b, const Params &a,
                                                                const Plan &plan, const Block &k, uint32_t kv_head,
                                                                uint32_t from, uint32_t to, int place, uint32_t share,
-                                                               Shared<HD, QT> &sh, const T *q, T *out) {
-    constexpr uint32_t kQueries = 16 * QT;
-    const uint32_t t = threadIdx.x;
+                                                               Shared<HD, M> &sh, const T *q, T *out) {
+    constexpr uint32_t kQueries = Mode<M>::queries;
+    constexpr int QT = Mode<M>::columns;
+    // (opaque: what follows from the lane is computed here again for each block, where the
+    // compiler would hold all of it in registers for the whole kernel, and spill)
+    uint32_t t = threadIdx.x;
+    asm volatile("" : "+v"(t));
     const uint32_t wave = __builtin_amdgcn_readfirstlane(t / 64), lane = t % 64, n = lane % 16, g = lane / 16;
-    const int32_t *const table = b.table + size_t(k.sequence) * b.stride;
+    Source<TP> src;
+    src.table = b.table + size_t(k.sequence) * b.stride;
+    src.page_bytes = size_t(c.kv_heads) * c.record;
+    src.head = c.pool + size_t(kv_head) * c.record;
+    src.lo = k.lo;
+    src.hi = k.hi;
+    src.last_min = uint32_t(max(k.position0 + int32_t(k.query0 / a.group), 0));
+    src.first_max = a.window && k.hi + 1 > a.window ? k.hi + 1 - a.window : 0;
     const uint32_t end = k.first_chunk + min(k.chunks, to * kWaves);
     const uint32_t first = k.first_chunk + from * kWaves + wave;
 
-    Wave<HD, QT, kQueryPlanes<T>> w;
+    Wave<HD, M, kQueryPlanes<T>> w;
     Places<TP> here{}, next{};
     Codes<HD> kc, vc;
     // everything that the first chunk needs is requested before anything is waited for
     if (first < end) {
-        here = places_of<TP>(c, table, first, k.lo, k.hi);
-        next = places_of<TP>(c, table, min(first + kWaves, end - 1), k.lo, k.hi);
+        here = src.places(c, first);
+        next = src.places(c, min(first + kWaves, end - 1));
     }
     RawQuery<HD, T> raw[QT];
 #pragma unroll
     for (int qi = 0; qi < QT; ++qi) {
-        const uint32_t query = k.query0 + 16 * qi + n, token = k.rows == 1 ? 0u : query / a.group;
+        const uint32_t query = k.query0 + (M == kHalf ? n % 8 : 16 * qi + n);
+        const uint32_t token = k.rows == 1 ? 0u : query / a.group;
         const bool there = query < k.rows * a.group;
         const int32_t position = k.position0 + int32_t(token);
         w.mine[qi].last = there ? position : -1;
@@ -733,7 +832,8 @@ __device__ __attribute__((always_inline)) inline void do_block(const Cache &c, c
         }
     }
     if (first < end) {
-        load_chunk<HD, TP>(c, kv_head, here, first, k.lo, k.hi, LaneOffsets<HD>(n, g), kc, vc);
+        load_codes<HD, TP, false>(c, src.head, src.page_bytes, here, first, src.lo, src.hi, LaneOffsets<HD>(n, g), kc);
+        load_codes<HD, TP, true>(c, src.head, src.page_bytes, here, first, src.lo, src.hi, LaneOffsets<HD>(n, g), vc);
     }
 #pragma unroll
     for (int qi = 0; qi < QT; ++qi) {
@@ -741,17 +841,15 @@ __device__ __attribute__((always_inline)) inline void do_block(const Cache &c, c
     }
     if (first < end) {
         uint16_t *const lds = sh.v[wave];
-        const uint32_t at = walk<HD, T, QT, TP, false>(c, a, k, table, kv_head, first, end, kc, vc, here, next, lds, n, g,
-                                                       w);
+        const uint32_t at = walk<HD, T, M, TP, false>(c, a, src, first, end, kc, vc, here, next, lds, n, g, w);
         if (at < end) {
-            Wave<HD, QT, kQueryPlanes<T>> copy = w;  // (the state itself stays in registers)
-            walk_odd<HD, T, QT, TP>(c, a, k, table, kv_head, at, end, lds, n, g, copy);
-            w = copy;
+            walk_odd<HD, T, M, TP>(c, a, src, at, end, lds, n, g, w);
         }
     }
 
-    // the waves' states joined through LDS
+    // the columns' states joined through LDS
     __syncthreads();
+    asm volatile("" : "+v"(t));
 #pragma unroll
     for (int qi = 0; qi < QT; ++qi) {
         const uint32_t poison = or_over_groups(w.nan_blocks[qi]);
@@ -775,19 +873,20 @@ __device__ __attribute__((always_inline)) inline void do_block(const Cache &c, c
         if (query >= k.rows * a.group) {
             break;
         }
-        float top = sh.join.b[0][local];
+        float top = -INFINITY;
 #pragma unroll
-        for (uint32_t x = 1; x < kWaves; ++x) {
-            top = fmaxf(top, sh.join.b[x][local]);
+        for (uint32_t x = 0; x < kWaves * Mode<M>::halves; ++x) {
+            top = fmaxf(top, sh.join.b[x % kWaves][local + x / kWaves * 8]);
         }
         const float base = top == -INFINITY ? 0.0f : top;
         f32x4 o = {0.f, 0.f, 0.f, 0.f};
         float l = 0.0f;
 #pragma unroll
-        for (uint32_t x = 0; x < kWaves; ++x) {
-            const float f = __builtin_amdgcn_exp2f(sh.join.b[x][local] - base);
-            const f32x4 y = *reinterpret_cast<const f32x4 *>(&sh.join.o[x][local][d]);
-            l = fmaf(sh.join.l[x][local], f, l);
+        for (uint32_t x = 0; x < kWaves * Mode<M>::halves; ++x) {
+            const uint32_t column = local + x / kWaves * 8;
+            const float f = __builtin_amdgcn_exp2f(sh.join.b[x % kWaves][column] - base);
+            const f32x4 y = *reinterpret_cast<const f32x4 *>(&sh.join.o[x % kWaves][column][d]);
+            l = fmaf(sh.join.l[x % kWaves][column], f, l);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 o[j] = fmaf(y[j], f, o[j]);
@@ -823,11 +922,11 @@ __device__ inline void fill_block(const Params &a, uint32_t queries, const Block
     }
 }
 
-template <int HD, class T, int QT, int TP>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kResident<HD, T, QT>))) void
+template <int HD, class T, int M, int TP>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kResident<HD, T, M>))) void
 attention_split_kernel(Cache c, Batch b, Params a, Plan plan, const T *__restrict__ q, T *__restrict__ out) {
-    constexpr uint32_t kQueries = 16 * QT;
-    __shared__ __attribute__((aligned(16))) Shared<HD, QT> sh;
+    constexpr uint32_t kQueries = Mode<M>::queries;
+    __shared__ __attribute__((aligned(16))) Shared<HD, M> sh;
     const uint32_t share = blockIdx.x, kv_head = blockIdx.y, t = threadIdx.x;
     uint32_t block = share, unit = 0, from = 0, to = 1;  // the block, its first unit, and the share's units
     uint64_t total = 0;
@@ -900,7 +999,7 @@ attention_split_kernel(Cache c, Batch b, Params a, Plan plan, const T *__restric
                 const uint64_t last = (uint64_t(unit) + units) * shares - 1;
                 plan.span[block] = make_uint2(share, uint32_t(last / total));
             }
-            do_block<HD, T, QT, TP>(c, b, a, plan, k, kv_head, x - unit, y - unit, place, share, sh, q, out);
+            do_block<HD, T, M, TP>(c, b, a, plan, k, kv_head, x - unit, y - unit, place, share, sh, q, out);
             __syncthreads();
         }
         unit += units;
@@ -1019,20 +1118,17 @@ int check_attention(const ttl_kv4_cache *cache, const ttl_kv4_batch *batch, cons
     return TTL_OK;
 }
 
-uint32_t resident_groups(uint32_t head_dim, int dtype, uint32_t tiles) {
+template <int M>
+uint32_t resident_groups(uint32_t head_dim, int dtype) {
     const bool f32 = dtype == TTL_DTYPE_F32;
-    if (head_dim == 64) {
-        return tiles == 2 ? (f32 ? kResident<64, float, 2> : kResident<64, __bf16, 2>)
-                          : (f32 ? kResident<64, float, 1> : kResident<64, __bf16, 1>);
-    }
-    return tiles == 2 ? (f32 ? kResident<128, float, 2> : kResident<128, __bf16, 2>)
-                      : (f32 ? kResident<128, float, 1> : kResident<128, __bf16, 1>);
+    return head_dim == 64 ? (f32 ? kResident<64, float, M> : kResident<64, __bf16, M>)
+                          : (f32 ? kResident<128, float, M> : kResident<128, __bf16, M>);
 }
 
-// The cut of a checked call: query tiles of a wave by the queries a sequence has on average, a
+// The cut of a checked call: the columns' use by the queries a sequence has on average, a
 // share for every workgroup that the card's 256 CUs hold at once.
 struct Cut {
-    uint32_t tiles;
+    int mode;
     Plan plan;
     uint32_t most_parts;  // of a block
     size_t workspace;
@@ -1042,9 +1138,9 @@ Cut cut_of(const ttl_kv4_cache *cache, const ttl_kv4_batch *batch, const ttl_kv4
     Cut cut{};
     const uint64_t queries = uint64_t(batch->tokens) * group;  // of a key/value head
     const uint64_t mean = queries / batch->sequences;
-    cut.tiles = mean > 16 ? 2 : 1;
+    cut.mode = mean > 16 ? kTwo : mean > 8 ? kOne : kHalf;
     Plan &p = cut.plan;
-    p.queries = 16 * cut.tiles;
+    p.queries = cut.mode == kTwo ? 32 : cut.mode == kOne ? 16 : 8;
     p.blocks = batch->starts ? uint32_t(queries / p.queries + batch->sequences)
                              : batch->sequences * ((group + p.queries - 1) / p.queries);
     uint32_t longest = batch->max_length;
@@ -1059,7 +1155,9 @@ Cut cut_of(const ttl_kv4_cache *cache, const ttl_kv4_batch *batch, const ttl_kv4
         p.shares = p.blocks;
         return cut;
     }
-    const uint32_t resident = resident_groups(cache->head_dim, attention->dtype, cut.tiles);
+    const uint32_t resident = cut.mode == kHalf  ? resident_groups<kHalf>(cache->head_dim, attention->dtype)
+                              : cut.mode == kOne ? resident_groups<kOne>(cache->head_dim, attention->dtype)
+                                                 : resident_groups<kTwo>(cache->head_dim, attention->dtype);
     p.shares = std::max(1u, 256 * resident / cache->kv_heads);
     p.shares = uint32_t(std::min<uint64_t>(p.shares, units * p.blocks));
     // a block spans the shares of its units
@@ -1119,22 +1217,24 @@ int run_attention(ttl_ctx *ctx, const ttl_kv4_cache *cache, const ttl_kv4_batch 
         T *ot = static_cast<T *>(out);
         const dim3 grid(p.shares, c.kv_heads);
         const bool big = c.page_shift >= 6;
-        const auto split = [&](auto tiles) {
-            constexpr int QT = decltype(tiles)::value;
+        const auto split = [&](auto mode) {
+            constexpr int M = decltype(mode)::value;
             if (big) {
-                attention_split_kernel<HD, T, QT, 1><<<grid, kThreads, 0, ctx->stream>>>(c, b, a, p, qt, ot);
+                attention_split_kernel<HD, T, M, 1><<<grid, kThreads, 0, ctx->stream>>>(c, b, a, p, qt, ot);
             } else {
-                attention_split_kernel<HD, T, QT, 4><<<grid, kThreads, 0, ctx->stream>>>(c, b, a, p, qt, ot);
+                attention_split_kernel<HD, T, M, 4><<<grid, kThreads, 0, ctx->stream>>>(c, b, a, p, qt, ot);
             }
         };
-        if (cut.tiles == 1) {
-            split(std::integral_constant<int, 1>());
+        if (cut.mode == kHalf) {
+            split(std::integral_constant<int, kHalf>());
+        } else if (cut.mode == kOne) {
+            split(std::integral_constant<int, kOne>());
         } else {
-            split(std::integral_constant<int, 2>());
+            split(std::integral_constant<int, kTwo>());
         }
         if (!p.single) {
             const size_t rows = size_t(b.tokens) * a.heads;
-            if (cut.most_parts > 16 && rows <= 4096) {
+            if (cut.most_parts > 16 && rows <= 1024) {
                 attention_join_kernel<HD, T, 4><<<uint32_t(rows), kThreads, 0, ctx->stream>>>(c, b, a, p, ot);
             } else {
                 attention_join_kernel<HD, T, 1><<<ttl::blocks_for(rows, kWaves), kThreads, 0, ctx->stream>>>(c, b, a, p,
