@@ -52,11 +52,11 @@ constexpr float kWeightShift = 11.0f;                               // weights a
 
 // How a wave's 16 columns are used (M): kHalf for 8 queries or fewer, columns 8..15 the same
 // queries on the other half of the chunk (so that no lane weighs scores that nobody asked for);
-// kOne and kTwo for 16 queries, and 32 in two column tiles.
-constexpr int kHalf = 0, kOne = 1, kTwo = 2;
+// kOne, kTwo and kFour for 16 queries, and 32 and 64 in two and four column tiles.
+constexpr int kHalf = 0, kOne = 1, kTwo = 2, kFour = 4;
 template <int M>
 struct Mode {
-    static constexpr int columns = M == kTwo ? 2 : 1;             // column tiles
+    static constexpr int columns = M == kHalf ? 1 : M;            // column tiles
     static constexpr int halves = M == kHalf ? 2 : 1;
     static constexpr int tiles = 4 / halves;                      // position tiles of a lane's column
     static constexpr uint32_t queries = M == kHalf ? 8 : 16 * columns;
@@ -71,14 +71,14 @@ struct Params {
 };
 
 // How a call is cut.  A block is up to `queries` queries of a sequence and key/value head; its
-// chunks count in units of kWaves, one chunk a wave.  The units of all blocks in a row are
+// chunks count in units of `unit`.  The units of all blocks in a row are
 // divided evenly among `shares` workgroups per key/value head, whatever the lengths are: a share
 // takes the end of one block, whole ones, and the beginning of another.  A block that one
 // share has whole is written by it; of the others every share leaves its part in `o` and `bl`
 // (place 1 where it holds the block's beginning, 0 elsewhere) for the join.
 struct Plan {
-    uint32_t queries, blocks, shares;
-    bool single;   // no block has more than one unit: a share is a block, nothing is joined
+    uint32_t queries, blocks, shares, unit;
+    bool single;   // a share is a block, nothing is joined
     float *o;      // [kv head][share][2][queries][HD]
     float2 *bl;    // [kv head][share][2][queries]: offset, sum
     uint2 *span;   // [block]: its first and last share
@@ -93,7 +93,6 @@ struct Block {
     uint32_t first_chunk, chunks;      // none: no row of the block sees a position
     uint32_t lo, hi;                   // the positions that its rows see
     bool exists, bad;
-    __device__ uint32_t units() const { return (chunks + kWaves - 1) / kWaves; }
 };
 
 __device__ inline Block block_span(const Batch &b, const Params &a, uint32_t queries, Block k) {
@@ -110,6 +109,10 @@ __device__ inline Block block_span(const Batch &b, const Params &a, uint32_t que
         k.chunks = k.hi / kChunk - k.first_chunk + 1;
     }
     return k;
+}
+
+__device__ inline uint32_t units_of(const Plan &plan, const Block &k) {
+    return plan.unit == 1 ? k.chunks : (k.chunks + kWaves - 1) / kWaves;
 }
 
 // Block `index` of a key/value head.  Sequence s of a ragged batch has its blocks from index
@@ -758,6 +761,11 @@ __device__ __attribute__((always_inline)) inline void walk_odd(const Cache &c, c
     walk<HD, T, M, TP, true>(c, a, src, chunk, end, kc, vc, here, next, lds, n, g, w);
 }
 
+struct ShareScan {
+    uint32_t sum[kWaves];
+    uint32_t block, first;  // the share's first block, and that block's first unit
+};
+
 // Workgroups of a CU (waves of a SIMD).  More would fit on 128 registers with M kHalf, and were
 // slower: 4 instead of 3 for bf16 queries 51.8 against 49.8 us (64 ragged sequences up to
 // 8192), 3 instead of 2 for f32 79.9 against 74.1 us (128 at 4096).
@@ -772,10 +780,7 @@ union Shared {
         float o[kWaves][16 * Mode<M>::columns][kOStride];
         float b[kWaves][16 * Mode<M>::columns], l[kWaves][16 * Mode<M>::columns];
     } join;
-    struct {
-        uint32_t sum[kWaves];
-        uint32_t block, first;  // the share's first block, and that block's first unit
-    } scan;
+    ShareScan scan;
 };
 
 // Units [from, to) of a block: the waves take its chunks in turn, and their states are joined.
@@ -922,89 +927,367 @@ __device__ inline void fill_block(const Params &a, uint32_t queries, const Block
     }
 }
 
-template <int HD, class T, int M, int TP>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kResident<HD, T, M>))) void
-attention_split_kernel(Cache c, Batch b, Params a, Plan plan, const T *__restrict__ q, T *__restrict__ out) {
-    constexpr uint32_t kQueries = Mode<M>::queries;
-    __shared__ __attribute__((aligned(16))) Shared<HD, M> sh;
+// The part of a share that lies in `block`s, one after the other: `work(k, from, to, place)` does
+// units [from, to) of block k.  Called by every thread of a workgroup.
+template <int HD, class T, class Work>
+__device__ __attribute__((always_inline)) inline void do_share(const Batch &b, const Params &a, const Plan &plan,
+                                                               ShareScan &scan, T *out, const Work &work) {
     const uint32_t share = blockIdx.x, kv_head = blockIdx.y, t = threadIdx.x;
-    uint32_t block = share, unit = 0, from = 0, to = 1;  // the block, its first unit, and the share's units
-    uint64_t total = 0;
-    uint32_t shares = 0;
-    if (!plan.single) {
-        // every workgroup sums up all blocks' units, and finds where its share begins
-        const uint32_t wave = t / 64, lane = t % 64;
-        const uint32_t per = (plan.blocks + kThreads - 1) / kThreads, first = t * per;
-        uint32_t mine = 0;
-        for (uint32_t i = first; i < min(first + per, plan.blocks); ++i) {
-            mine += block_of(b, a, kQueries, i).units();
+    if (plan.single) {
+        // (the blocks with the most positions come last: first of all)
+        const Block k = block_of(b, a, plan.queries, plan.shares - 1 - share);
+        if (k.chunks) {
+            work(k, 0u, units_of(plan, k), -1);
+        } else if (k.exists) {
+            fill_block<HD, T>(a, plan.queries, k, kv_head, out);
         }
-        uint32_t sum = mine;  // of the lanes up to this one
-#pragma unroll
-        for (uint32_t d = 1; d < 64; d <<= 1) {
-            const uint32_t x = __shfl_up(sum, d);
-            sum += lane >= d ? x : 0u;
-        }
-        if (lane == 63) {
-            sh.scan.sum[wave] = sum;
-        }
-        __syncthreads();
-        uint32_t before = sum - mine;
-#pragma unroll
-        for (uint32_t w = 0; w < kWaves; ++w) {
-            const uint32_t x = sh.scan.sum[w];
-            before += w < wave ? x : 0u;
-            total += x;
-        }
-        shares = uint32_t(min(uint64_t(plan.shares), total));  // a unit each at least
-        if (share >= shares) {
-            return;
-        }
-        from = uint32_t(total * share / shares);
-        to = uint32_t(total * (share + 1) / shares);
-        if (from >= before && from < before + mine) {
-            uint32_t at = before, i = first;
-            while (true) {
-                const uint32_t n = block_of(b, a, kQueries, i).units();
-                if (from < at + n) {
-                    break;
-                }
-                at += n;
-                ++i;
-            }
-            sh.scan.block = i;
-            sh.scan.first = at;
-        }
-        __syncthreads();
-        block = __builtin_amdgcn_readfirstlane(sh.scan.block);
-        unit = __builtin_amdgcn_readfirstlane(sh.scan.first);
-        __syncthreads();
+        return;
     }
-    while (unit < to) {
-        const Block k = block_of(b, a, kQueries, block);
-        const uint32_t units = k.units();
-        if (plan.single) {
-            if (units == 0) {
-                if (k.exists) {
-                    fill_block<HD, T>(a, kQueries, k, kv_head, out);
-                }
-                return;
+    // every workgroup sums up all blocks' units, and finds where its share begins
+    const uint32_t wave = t / 64, lane = t % 64;
+    const uint32_t per = (plan.blocks + kThreads - 1) / kThreads, mine0 = t * per;
+    uint32_t mine = 0;
+    for (uint32_t i = mine0; i < min(mine0 + per, plan.blocks); ++i) {
+        mine += units_of(plan, block_of(b, a, plan.queries, i));
+    }
+    uint32_t sum = mine;  // of the lanes up to this one
+#pragma unroll
+    for (uint32_t d = 1; d < 64; d <<= 1) {
+        const uint32_t x = __shfl_up(sum, d);
+        sum += lane >= d ? x : 0u;
+    }
+    if (lane == 63) {
+        scan.sum[wave] = sum;
+    }
+    __syncthreads();
+    uint32_t before = sum - mine;
+    uint64_t total = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kWaves; ++w) {
+        const uint32_t x = scan.sum[w];
+        before += w < wave ? x : 0u;
+        total += x;
+    }
+    const uint32_t shares = uint32_t(min(uint64_t(plan.shares), total));  // a unit each at least
+    if (share >= shares) {
+        return;
+    }
+    const uint32_t from = uint32_t(total * share / shares), to = uint32_t(total * (share + 1) / shares);
+    if (from >= before && from < before + mine) {
+        uint32_t at = before, i = mine0;
+        while (true) {
+            const uint32_t n = units_of(plan, block_of(b, a, plan.queries, i));
+            if (from < at + n) {
+                break;
             }
+            at += n;
+            ++i;
         }
+        scan.block = i;
+        scan.first = at;
+    }
+    __syncthreads();
+    uint32_t block = __builtin_amdgcn_readfirstlane(scan.block), unit = __builtin_amdgcn_readfirstlane(scan.first);
+    __syncthreads();
+    while (unit < to) {
+        const Block k = block_of(b, a, plan.queries, block);
+        const uint32_t units = units_of(plan, k);
         if (units) {
             const uint32_t x = max(from, unit), y = min(to, unit + units);
             const int place = x == unit && y == unit + units ? -1 : x == unit ? 1 : 0;
-            if (place != 0 && !plan.single && kv_head == 0 && t == 0) {
+            if (place != 0 && kv_head == 0 && t == 0) {
                 // the share of a unit u is the last one that begins at u or before
                 const uint64_t last = (uint64_t(unit) + units) * shares - 1;
                 plan.span[block] = make_uint2(share, uint32_t(last / total));
             }
-            do_block<HD, T, M, TP>(c, b, a, plan, k, kv_head, x - unit, y - unit, place, share, sh, q, out);
+            work(k, x - unit, y - unit, place);
             __syncthreads();
         }
         unit += units;
         ++block;
     }
+}
+
+template <int HD, class T, int M, int TP>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kResident<HD, T, M>))) void
+attention_split_kernel(Cache c, Batch b, Params a, Plan plan, const T *__restrict__ q, T *__restrict__ out) {
+    __shared__ __attribute__((aligned(16))) Shared<HD, M> sh;
+    do_share<HD, T>(b, a, plan, sh.scan, out, [&](const Block &k, uint32_t from, uint32_t to, int place) {
+        do_block<HD, T, M, TP>(c, b, a, plan, k, blockIdx.y, from, to, place, blockIdx.x, sh, q, out);
+    });
+}
+
+// ---- many queries: the waves of a workgroup share the chunks, each with queries of its own --------
+//
+// Each wave converts a tile of 16 positions of the chunk, K to bf16 and V to f16 in LDS, where
+// all four read it; two buffers, so that the next chunk is converted while this one is used,
+// with one barrier a chunk.  A chunk with values outside the f16 path's range is found when it
+// is converted (a flag a wave, beside the buffer) and then converted again, for the bf16 path.
+
+template <int HD>
+struct TileShared {
+    union {
+        struct {
+            uint16_t k[2][kChunk * kVStride<HD>], v[2][kChunk * kVStride<HD>];
+        };
+        ShareScan scan;
+    };
+    uint32_t far[2][kWaves];
+};
+
+// One tile of a chunk's codes (position n, a quarter of the head).
+template <int HD>
+struct TileCodes {
+    uint32_t kw[HD / 32], vw[HD / 32], ks, vs;
+};
+
+template <int HD, int TP>
+__device__ __attribute__((always_inline)) inline void load_tile(const Cache &c, const Source<TP> &src, uint32_t chunk,
+                                                                uint32_t page, uint32_t wave,
+                                                                const LaneOffsets<HD> &at, TileCodes<HD> &x) {
+    using L = Layout<HD>;
+    const uint32_t tile = TP == 1 ? chunk * kTiles + wave : min(max(chunk * kTiles + wave, src.lo / 16), src.hi / 16);
+    const uint32_t slot = (tile * 16) & ((1u << c.page_shift) - 1);
+    const uint8_t *rec = src.head + (page < c.pages ? page : 0u) * src.page_bytes;  // uniform
+    load_words<HD>(rec + L::k_codes(slot) + at.code, x.kw);
+    load_words<HD>(rec + L::v_codes(c.page_shift, slot) + at.code, x.vw);
+    x.ks = (rec + L::k_scales(c.page_shift, slot))[at.scale];
+    x.vs = (rec + L::v_scales(c.page_shift, slot))[at.scale];
+}
+
+// The page of a wave's tile of a chunk.
+template <int TP>
+__device__ __attribute__((always_inline)) inline uint32_t tile_page(const Cache &c, const Source<TP> &src,
+                                                                    uint32_t chunk, uint32_t wave) {
+    const uint32_t tile = TP == 1 ? chunk * kTiles : min(max(chunk * kTiles + wave, src.lo / 16), src.hi / 16);
+    return uint32_t(kv4::entry(src.table, tile >> (c.page_shift - 4)));
+}
+
+template <int HD, class V>
+__device__ __attribute__((always_inline)) inline void stage_row(uint16_t *row, const uint32_t (&w)[HD / 32],
+                                                                uint32_t scale) {
+#pragma unroll
+    for (int s = 0; s < HD / 32; ++s) {
+        *reinterpret_cast<V *>(row + 8 * s) = mf::decode_as<V>(w[s], kv4::scale_of(scale));
+    }
+}
+
+template <int HD, class T, int M, int TP>
+__device__ __attribute__((always_inline)) inline void do_tile(const Cache &c, const Batch &b, const Params &a,
+                                                              const Plan &plan, const Block &k, uint32_t kv_head,
+                                                              uint32_t from, uint32_t to, int place, uint32_t share,
+                                                              TileShared<HD> &sh, const T *q, T *out) {
+    constexpr int QT = Mode<M>::columns, NS = HD / 32, QP = kQueryPlanes<T>, PP = kWeightPlanes<T>;
+    uint32_t t = threadIdx.x;
+    asm volatile("" : "+v"(t));  // (as in do_block)
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(t / 64), lane = t % 64, n = lane % 16, g = lane / 16;
+    Source<TP> src;
+    src.table = b.table + size_t(k.sequence) * b.stride;
+    src.page_bytes = size_t(c.kv_heads) * c.record;
+    src.head = c.pool + size_t(kv_head) * c.record;
+    src.lo = k.lo;
+    src.hi = k.hi;
+    const LaneOffsets<HD> at(n, g);
+    const uint32_t first = k.first_chunk + from, end = k.first_chunk + to;
+
+    // the wave's own queries: which, what they see, and what all and any of them see
+    State<HD, M> st;
+    bf16x8 qf[QT][NS][QP];
+    Query mine[QT];
+    uint32_t nan_blocks[QT];
+    const uint32_t own = k.query0 + wave * (16 * QT), limit = k.rows * a.group;
+    const uint32_t own_last = min(own + 16 * QT, limit) - 1;
+    const bool any = own < limit;
+    const int32_t p0 = k.position0 + int32_t((any ? own : 0u) / a.group);
+    const int32_t p1 = k.position0 + int32_t((any ? own_last : 0u) / a.group);
+    const int32_t window = a.window ? int32_t(a.window) : INT32_MAX;
+    const int32_t first_min = max(p0 + 1 - window, 0), first_max = max(p1 + 1 - window, 0);  // (p <= 2^30)
+#pragma unroll
+    for (int qi = 0; qi < QT; ++qi) {
+        const uint32_t query = own + 16 * qi + n, token = query / a.group;
+        const bool there = query < limit;
+        const int32_t position = k.position0 + int32_t(token);
+        mine[qi].last = there ? position : -1;
+        mine[qi].first = max(position + 1 - window, 0);
+        const uint32_t row = k.row0 + (there ? token : 0u);
+        const uint32_t head = kv_head * a.group + (there ? query - token * a.group : 0u);
+        RawQuery<HD, T> raw;
+        raw.load(q + (size_t(row) * a.heads + head) * HD, g);
+        raw.planes(a.negate, qf[qi]);
+        st.b[qi] = -INFINITY;
+        st.l[qi] = 0.0f;
+        nan_blocks[qi] = 0;
+#pragma unroll
+        for (int mt = 0; mt < HD / 16; ++mt) {
+            st.o[qi][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+
+    TileCodes<HD> x;
+    // positions of the tile outside lo..hi, and pages that are not there
+    const auto trim = [&](uint32_t chunk, uint32_t page) __attribute__((always_inline)) {
+        const uint32_t p = chunk * kChunk + 16 * wave + n;
+        const bool inside = chunk * kChunk >= src.lo && chunk * kChunk + kChunk - 1 <= src.hi;
+        if (!inside || page >= c.pages) {
+            const bool zero = p < src.lo || p > src.hi || page >= c.pages;
+            x.ks = page >= c.pages ? 255u : x.ks;
+            x.vs = zero ? 127u : x.vs;
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                x.vw[s] = zero ? 0u : x.vw[s];
+            }
+        }
+    };
+    const auto stage = [&](uint32_t chunk, uint32_t page) __attribute__((always_inline)) {
+        trim(chunk, page);
+        const uint32_t buf = chunk % 2, row = (16 * wave + n) * kVStride<HD> + g * (HD / 4);
+        stage_row<HD, bf16x8>(sh.k[buf] + row, x.kw, x.ks);
+        stage_row<HD, f16x8>(sh.v[buf] + row, x.vw, x.vs);
+        const bool far = __any(x.vs - kF16First > kF16Last - kF16First);
+        if (lane == 0) {
+            sh.far[buf][wave] = far ? 1u : 0u;
+        }
+    };
+    uint32_t page = tile_page<TP>(c, src, first, wave);
+    uint32_t next = tile_page<TP>(c, src, min(first + 1, end - 1), wave);
+    load_tile<HD, TP>(c, src, first, page, wave, at, x);
+    stage(first, page);
+    page = next;
+    next = tile_page<TP>(c, src, min(first + 2, end - 1), wave);
+    load_tile<HD, TP>(c, src, min(first + 1, end - 1), page, wave, at, x);
+    __syncthreads();
+
+#pragma unroll 1
+    for (uint32_t chunk = first; chunk < end; ++chunk) {
+        const uint32_t buf = chunk % 2;
+        const int32_t c0 = int32_t(chunk * kChunk);
+        const bool far = (sh.far[buf][0] | sh.far[buf][1] | sh.far[buf][2] | sh.far[buf][3]) != 0;
+        // (every thread sees the same flags: all of them take the same way, with its barriers)
+        const bool odd = __builtin_amdgcn_readfirstlane(uint32_t(far)) != 0;
+        const bool needed = any && c0 <= p1 && c0 + int32_t(kChunk) > first_min;
+        const bool whole = c0 >= first_max && c0 + int32_t(kChunk) - 1 <= p0;
+        f32x4 s[QT][kTiles];
+        if (needed) {
+            const uint16_t *const ks = sh.k[buf] + n * kVStride<HD> + g * (HD / 4);
+#pragma unroll
+            for (int step = 0; step < NS; ++step) {
+                bf16x8 kf[kTiles];
+#pragma unroll
+                for (uint32_t i = 0; i < kTiles; ++i) {
+                    kf[i] = *reinterpret_cast<const bf16x8 *>(ks + 16 * i * kVStride<HD> + 8 * step);
+                }
+#pragma unroll
+                for (int p = QP - 1; p >= 0; --p) {
+#pragma unroll
+                    for (uint32_t i = 0; i < kTiles; ++i) {
+#pragma unroll
+                        for (int qi = 0; qi < QT; ++qi) {
+                            s[qi][i] = mf::mfma(kf[i], qf[qi][step][p],
+                                                step == 0 && p == QP - 1 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[qi][i]);
+                        }
+                    }
+                }
+            }
+        }
+        // the next chunk into the other buffer, whose readers are behind the last barrier
+        if (chunk + 1 < end) {
+            stage(chunk + 1, page);
+            page = next;
+            next = tile_page<TP>(c, src, min(chunk + 3, end - 1), wave);
+            load_tile<HD, TP>(c, src, min(chunk + 2, end - 1), page, wave, at, x);
+        }
+        if (needed) {
+#pragma unroll
+            for (int qi = 0; qi < QT; ++qi) {
+                softmax_step<HD, M>(s[qi], st, qi, mine[qi], whole, c0 + int32_t(4 * g), a.c);
+            }
+            if (!odd) {
+                weigh_values<HD, f16x8, PP, M>(sh.v[buf], s, st, n, g);
+            }
+        }
+        if (odd) {
+            // V again, as bf16, its NaN blocks as zeros and a bit each behind their row
+            __syncthreads();
+            const uint32_t here = tile_page<TP>(c, src, chunk, wave);
+            const TileCodes<HD> keep = x;
+            load_tile<HD, TP>(c, src, chunk, here, wave, at, x);
+            trim(chunk, here);
+            const bool nan = x.vs == 255;
+            const uint32_t bits = or_over_groups(nan ? 1u << (g * (HD / 4) / 32) : 0u);
+            uint16_t *const row = sh.v[buf] + (16 * wave + n) * kVStride<HD>;
+            if (g == 0) {
+                row[HD] = uint16_t(bits);
+            }
+            x.vs = nan ? 127u : x.vs;
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                x.vw[i] = nan ? 0u : x.vw[i];
+            }
+            stage_row<HD, bf16x8>(row + g * (HD / 4), x.vw, x.vs);
+            x = keep;
+            __syncthreads();
+            if (needed) {
+                weigh_values_odd<HD, M>(sh.v[buf], s, st, n, g);
+#pragma unroll
+                for (uint32_t i = 0; i < kTiles; ++i) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int32_t local = int32_t(16 * i + 4 * g) + j, p = c0 + local;
+                        const uint32_t nans = sh.v[buf][local * int32_t(kVStride<HD>) + HD];
+#pragma unroll
+                        for (int qi = 0; qi < QT; ++qi) {
+                            nan_blocks[qi] |= p >= mine[qi].first && p <= mine[qi].last ? nans : 0u;
+                        }
+                    }
+                }
+            }
+        }
+        __syncthreads();
+    }
+
+#pragma unroll
+    for (int qi = 0; qi < QT; ++qi) {
+        const uint32_t query = own + 16 * qi + n, token = query / a.group;
+        const uint32_t poison = or_over_groups(nan_blocks[qi]);
+        const float l = sum_over_groups(st.l[qi]);
+        if (query >= limit) {
+            continue;
+        }
+        const uint32_t head = kv_head * a.group + query - token * a.group;
+        const bool idle = k.position0 + int32_t(token) < 0;
+#pragma unroll
+        for (int mt = 0; mt < HD / 16; ++mt) {
+            f32x4 o = st.o[qi][mt];
+            if (poison >> (mt / 2) & 1) {
+                o = f32x4{__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+            }
+            const uint32_t d = 16 * mt + 4 * g;
+            if (place < 0) {
+                store4(out + (size_t(k.row0 + token) * a.heads + head) * HD + d,
+                       idle ? f32x4{0.f, 0.f, 0.f, 0.f} : with_sink(a, head, st.b[qi], o, l));
+            } else {
+                const size_t to_place =
+                    ((size_t(kv_head) * plan.shares + share) * 2 + uint32_t(place)) * plan.queries + (query - k.query0);
+                *reinterpret_cast<f32x4 *>(plan.o + to_place * HD + d) = o;
+                if (d == 0) {
+                    plan.bl[to_place] = make_float2(st.b[qi], l);
+                }
+            }
+        }
+    }
+}
+
+// Workgroups of a CU.
+template <int HD, class T, int M>
+constexpr int kTileResident = HD == 128 && std::is_same<T, float>::value ? 1 : 2;
+
+template <int HD, class T, int M, int TP>
+__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kTileResident<HD, T, M>))) void
+attention_tile_kernel(Cache c, Batch b, Params a, Plan plan, const T *__restrict__ q, T *__restrict__ out) {
+    __shared__ __attribute__((aligned(16))) TileShared<HD> sh;
+    do_share<HD, T>(b, a, plan, sh.scan, out, [&](const Block &k, uint32_t from, uint32_t to, int place) {
+        do_tile<HD, T, M, TP>(c, b, a, plan, k, blockIdx.y, from, to, place, blockIdx.x, sh, q, out);
+    });
 }
 
 // ---- the parts of a block joined ---------------------------------------------------------------
@@ -1125,22 +1408,42 @@ uint32_t resident_groups(uint32_t head_dim, int dtype) {
                           : (f32 ? kResident<128, float, M> : kResident<128, __bf16, M>);
 }
 
-// The cut of a checked call: the columns' use by the queries a sequence has on average, a
-// share for every workgroup that the card's 256 CUs hold at once.
+// The cut of a checked call, by the queries that a sequence has on average: few share a
+// workgroup's waves, from kTileFrom on each wave has its own.
 struct Cut {
+    bool tile;
     int mode;
     Plan plan;
     uint32_t most_parts;  // of a block
     size_t workspace;
 };
+constexpr uint64_t kTileFrom = 64;
+constexpr uint64_t kCus = 256;
 Cut cut_of(const ttl_kv4_cache *cache, const ttl_kv4_batch *batch, const ttl_kv4_attention *attention) {
     const uint32_t group = attention->heads / cache->kv_heads;
+    const bool f32 = attention->dtype == TTL_DTYPE_F32;
     Cut cut{};
     const uint64_t queries = uint64_t(batch->tokens) * group;  // of a key/value head
     const uint64_t mean = queries / batch->sequences;
-    cut.mode = mean > 16 ? kTwo : mean > 8 ? kOne : kHalf;
     Plan &p = cut.plan;
-    p.queries = cut.mode == kTwo ? 32 : cut.mode == kOne ? 16 : 8;
+    cut.tile = batch->starts && mean >= kTileFrom;
+    uint64_t slots;
+    if (cut.tile) {
+        // four column tiles a wave read K and V from LDS half as often as two do; two leave more
+        // workgroups
+        const bool four = false && !f32 && cache->head_dim == 64 && queries / 256 * cache->kv_heads >= 2 * kCus;
+        cut.mode = four ? kFour : kTwo;
+        p.queries = kWaves * 16 * uint32_t(cut.mode);
+        p.unit = 1;
+        slots = kCus * (cache->head_dim == 128 && f32 ? 1 : 2);
+    } else {
+        cut.mode = mean > 16 ? kTwo : mean > 8 ? kOne : kHalf;
+        p.queries = cut.mode == kTwo ? 32 : cut.mode == kOne ? 16 : 8;
+        p.unit = kWaves;
+        slots = kCus * (cut.mode == kHalf  ? resident_groups<kHalf>(cache->head_dim, attention->dtype)
+                        : cut.mode == kOne ? resident_groups<kOne>(cache->head_dim, attention->dtype)
+                                           : resident_groups<kTwo>(cache->head_dim, attention->dtype));
+    }
     p.blocks = batch->starts ? uint32_t(queries / p.queries + batch->sequences)
                              : batch->sequences * ((group + p.queries - 1) / p.queries);
     uint32_t longest = batch->max_length;
@@ -1149,16 +1452,15 @@ Cut cut_of(const ttl_kv4_cache *cache, const ttl_kv4_batch *batch, const ttl_kv4
         longest = uint32_t(std::min<uint64_t>(longest, uint64_t(attention->window) + p.queries / group + 1));
     }
     const uint32_t chunks = longest / kChunk + (attention->window ? 2 : 1);  // any alignment
-    const uint64_t units = (chunks + kWaves - 1) / kWaves;
-    p.single = units == 1;
+    const uint64_t units = (chunks + p.unit - 1) / p.unit;
+    // With enough blocks (or so many that finding a share would take long) a workgroup takes a
+    // block whole.
+    p.single = units == 1 || (cut.tile && uint64_t(p.blocks) * cache->kv_heads >= 2 * slots) || p.blocks > 1u << 16;
     if (p.single) {
         p.shares = p.blocks;
         return cut;
     }
-    const uint32_t resident = cut.mode == kHalf  ? resident_groups<kHalf>(cache->head_dim, attention->dtype)
-                              : cut.mode == kOne ? resident_groups<kOne>(cache->head_dim, attention->dtype)
-                                                 : resident_groups<kTwo>(cache->head_dim, attention->dtype);
-    p.shares = std::max(1u, 256 * resident / cache->kv_heads);
+    p.shares = uint32_t(std::max<uint64_t>(1, slots / cache->kv_heads));
     p.shares = uint32_t(std::min<uint64_t>(p.shares, units * p.blocks));
     // a block spans the shares of its units
     cut.most_parts = uint32_t(std::min<uint64_t>(p.shares, units + 1));
@@ -1225,7 +1527,24 @@ int run_attention(ttl_ctx *ctx, const ttl_kv4_cache *cache, const ttl_kv4_batch 
                 attention_split_kernel<HD, T, M, 4><<<grid, kThreads, 0, ctx->stream>>>(c, b, a, p, qt, ot);
             }
         };
-        if (cut.mode == kHalf) {
+        const auto tile = [&](auto mode) {
+            constexpr int M = decltype(mode)::value;
+            if (big) {
+                attention_tile_kernel<HD, T, M, 1><<<grid, kThreads, 0, ctx->stream>>>(c, b, a, p, qt, ot);
+            } else {
+                attention_tile_kernel<HD, T, M, 4><<<grid, kThreads, 0, ctx->stream>>>(c, b, a, p, qt, ot);
+            }
+        };
+        if (cut.tile) {
+            if constexpr (HD == 64 && !std::is_same<T, float>::value) {
+                if (cut.mode == kFour) {
+                    tile(std::integral_constant<int, kFour>());
+                }
+            }
+            if (cut.mode == kTwo) {
+                tile(std::integral_constant<int, kTwo>());
+            }
+        } else if (cut.mode == kHalf) {
             split(std::integral_constant<int, kHalf>());
         } else if (cut.mode == kOne) {
             split(std::integral_constant<int, kOne>());
