@@ -160,13 +160,13 @@ def allowance(ref, mag, smax, vsum, n, hd, bf16):
     each, relative to the sum of magnitudes; 32 more roundings for the rest (rescaling, joins,
     the sink, the division).  A bf16 output: the weights in f16 (2^-11) and the output's own
     rounding (2^-8).
-    Small weights: a score seen before (once the largest) has its weight held as 2^11, in f16,
+    Small weights: a score seen before (once the largest) has its weight held as 2^7, in f16,
     whose smallest step is 2^-24.  What the last f16 plane rounds off is at most half of it,
-    2^-25 / 2^11 = 2^-36 of that weight, which is at most 1 of the final sum: 2^-36 |v| for each
+    2^-25 / 2^7 = 2^-32 of that weight, which is at most 1 of the final sum: 2^-32 |v| for each
     position seen.  (It shows where the large weights meet a v of exactly zero, as one
     in eight E2M1 codes is.)  Below f32's smallest normal value bits of an output may be lost."""
     u = 2.0 ** -24
-    floor = 2.0 ** -36 * vsum + 2.0 ** -133
+    floor = 2.0 ** -32 * vsum + 2.0 ** -133
     rel = 2.0 * (hd + 8) * u * smax[..., None] + (2 * n + 32) * u
     if bf16:
         return mag * (rel + 2.0 ** -11) * 1.01 + 2.0 ** -8 * np.abs(ref) * 1.01 + floor

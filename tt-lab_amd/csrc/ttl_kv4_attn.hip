@@ -18,9 +18,9 @@
 // weights never leave their registers.
 //
 // Numerics: K and bf16 queries are exact in bf16, f32 queries three bf16 planes (24 bits).  The
-// weights, relative to a large one held as 2^11, are rounded to f16 for a bf16 output (2^-11, an
+// weights, relative to a large one held as 2^7, are rounded to f16 for a bf16 output (2^-11, an
 // eighth of the output's own rounding) and to two f16 planes for an f32 one (2^-22; weights
-// below 2^-25 of the large one lose more of themselves, 2^-36 of it).  V is exact in f16 where
+// below 2^-21 of the large one lose more of themselves, 2^-32 of it).  V is exact in f16 where
 // its scale bytes are 104..140 (subnormals included: the matrix cores keep them); a chunk with
 // another one takes V as bf16, exact for every byte, and three bf16 planes of the weights.
 // Maxima, sums and outputs are f32.
@@ -48,12 +48,12 @@ constexpr uint32_t kChunk = 64, kTiles = kChunk / 16;
 constexpr uint32_t kWaves = 4, kThreads = kWaves * 64;
 constexpr float kLog2e = 0x1.715476p+0f, kLog2eLo = 0x1.4ae0cp-26f;  // log2 e = their sum
 constexpr uint32_t kF16First = 104, kF16Last = 140;                  // scale bytes of V on the f16 path
-constexpr float kWeightShift = 11.0f;                               // weights are held times 2^11
+constexpr float kWeightShift = 7.0f;                                // weights are held times 2^7
 
 // How a wave's 16 columns are used (M): kHalf for 8 queries or fewer, columns 8..15 the same
 // queries on the other half of the chunk (so that no lane weighs scores that nobody asked for);
-// kOne, kTwo and kFour for 16 queries, and 32 and 64 in two and four column tiles.
-constexpr int kHalf = 0, kOne = 1, kTwo = 2, kFour = 4;
+// kOne and kTwo for 16 queries, and 32 in two column tiles.
+constexpr int kHalf = 0, kOne = 1, kTwo = 2;
 template <int M>
 struct Mode {
     static constexpr int columns = M == kHalf ? 1 : M;            // column tiles
@@ -267,7 +267,7 @@ __device__ __attribute__((always_inline)) inline bool all_in_pool(const Cache &c
 
 template <int HD, int M>
 struct State {
-    float b[Mode<M>::columns];  // offset: c x a large score - 11; weights are 2^(c s - b), 2^15 at most
+    float b[Mode<M>::columns];  // offset: c x a large score - 7; weights are 2^(c s - b), 2^15 at most
     float l[Mode<M>::columns];  // the lane's share of their sum
     f32x4 o[Mode<M>::columns][HD / 16];  // O^T: dims 16 mt + 4g + i of column n
 };
@@ -296,66 +296,74 @@ struct Query {
     int32_t first, last;
 };
 
-// Scores to weights.  The offset follows the largest score lazily: it is set anew (and what is
-// there rescaled) only when a lane's weights pass 2^15 together, before which none leaves
-// the f16 range, or before any score was seen (its weights are then infinite).
+// Scores to weights, in place.  The offset follows the largest score lazily: it is set anew (and
+// what is there rescaled) only when a weight would pass 2^15, before which none leaves the f16
+// range, or before any score was seen (its weights would then be infinite).
 // `at`: the position of the lane's first score.
 template <int HD, int M>
-__device__ __attribute__((always_inline)) inline void softmax_step(f32x4 (&s)[Mode<M>::tiles], State<HD, M> &st, int qi,
-                                                                   const Query &q, bool whole, int32_t at, float c) {
-    constexpr int NT = Mode<M>::tiles;
+__device__ __attribute__((always_inline)) inline void softmax_step(f32x4 (&s)[Mode<M>::columns][Mode<M>::tiles],
+                                                                   State<HD, M> &st,
+                                                                   const Query (&q)[Mode<M>::columns], bool whole,
+                                                                   int32_t at, float c) {
+    constexpr int NT = Mode<M>::tiles, QT = Mode<M>::columns;
     if (!whole) {
+        asm volatile("" : "+v"(at));  // (the positions are computed here, not for every chunk)
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
+        for (int qi = 0; qi < QT; ++qi) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int32_t p = at + 16 * i + j;
-                s[i][j] = p >= q.first && p <= q.last ? s[i][j] : -INFINITY;
+            for (int i = 0; i < NT; ++i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int32_t p = at + 16 * i + j;
+                    s[qi][i][j] = p >= q[qi].first && p <= q[qi].last ? s[qi][i][j] : -INFINITY;
+                }
             }
         }
     }
-    const auto weigh = [&](float base, f32x4 (&p)[NT]) __attribute__((always_inline)) {
-        f32x4 sum;
+    float m[QT];
+    bool far = false;
+#pragma unroll
+    for (int qi = 0; qi < QT; ++qi) {
+        m[qi] = s[qi][0][0];  // (fmaxf drops NaN scores; their weights are NaN all the same)
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                p[i][j] = __builtin_amdgcn_exp2f(fmaf(s[i][j], c, -base));
-                sum[j] = i ? sum[j] + p[i][j] : p[i][j];
+                m[qi] = fmaxf(m[qi], s[qi][i][j]);
             }
         }
-        return (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    };
-    f32x4 p[NT];
-    float sum = weigh(st.b[qi], p);
-    if (__any(!(sum <= 0x1p15f))) {
-        float m = s[0][0];
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                m = fmaxf(m, s[i][j]);
-            }
-        }
-        m = max_over_groups(m);
-        // fmaxf drops NaN scores; their weights are NaN all the same
-        const float b = fmaxf(st.b[qi], m == -INFINITY ? m : fmaf(m, c, -kWeightShift));
-        const float keep = b == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st.b[qi] - b);
-        st.b[qi] = b;
-        st.l[qi] *= keep;
-#pragma unroll
-        for (int mt = 0; mt < HD / 16; ++mt) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                st.o[qi][mt][j] *= keep;
-            }
-        }
-        sum = weigh(b == -INFINITY ? 0.0f : b, p);
+        far |= fmaf(m[qi], c, -st.b[qi]) > 15.0f;
     }
-    st.l[qi] += sum;
+    if (__any(far)) {
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-        s[i] = p[i];
+        for (int qi = 0; qi < QT; ++qi) {
+            const float x = max_over_groups(m[qi]);
+            const float b = fmaxf(st.b[qi], x == -INFINITY ? x : fmaf(x, c, -kWeightShift));
+            const float keep = b == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(st.b[qi] - b);
+            st.b[qi] = b;
+            st.l[qi] *= keep;
+#pragma unroll
+            for (int mt = 0; mt < HD / 16; ++mt) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    st.o[qi][mt][j] *= keep;
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int qi = 0; qi < QT; ++qi) {
+        const float base = st.b[qi] == -INFINITY ? 0.0f : st.b[qi];
+        f32x4 x;
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                s[qi][i][j] = __builtin_amdgcn_exp2f(fmaf(s[qi][i][j], c, -base));
+                x[j] = i ? x[j] + s[qi][i][j] : s[qi][i][j];
+            }
+        }
+        st.l[qi] += (x[0] + x[1]) + (x[2] + x[3]);
     }
 }
 
@@ -392,10 +400,14 @@ __device__ __attribute__((always_inline)) inline void split(const float (&x)[8],
 
 // ---- V through LDS --------------------------------------------------------------------------------
 
-// Row stride in 16-bit values: 16 more than the head, so that the four rows of a transposing
-// read (and the eight of a 16-byte store) fall into different banks.
+// Rows of HD 16-bit values, a row's 16-byte pieces in an order of their own, in which 16 rows of
+// a piece (16-byte stores and reads) and 8 rows of two neighbouring pieces (transposing reads)
+// lie in 64 different banks.  Where piece c of `row` begins, in values:
 template <int HD>
-constexpr uint32_t kVStride = HD + 16;
+__device__ __attribute__((always_inline)) inline uint32_t piece_at(uint32_t row, uint32_t c) {
+    const uint32_t turn = HD == 64 ? (row / 2) % 4 : row % 8;
+    return row * HD + (((c / 2) ^ turn) * 2 + ((c % 2) ^ (row / 8 % 2))) * 8;
+}
 
 template <int HD, class V>
 __device__ __attribute__((always_inline)) inline void stage_values(uint16_t *lds, const Codes<HD> &v, uint32_t n,
@@ -403,10 +415,11 @@ __device__ __attribute__((always_inline)) inline void stage_values(uint16_t *lds
 #pragma unroll
     for (uint32_t i = 0; i < kTiles; ++i) {
         const float scale = kv4::scale_of(v.scale[i]);
-        uint16_t *row = lds + (16 * i + n) * kVStride<HD> + g * (HD / 4);
 #pragma unroll
         for (int s = 0; s < HD / 32; ++s) {
-            *reinterpret_cast<V *>(row + 8 * s) = mf::decode_as<V>(v.w[i][s], scale);
+            // (rows 16 apart are turned alike)
+            *reinterpret_cast<V *>(lds + piece_at<HD>(n, g * (HD / 32) + s) + 16 * i * HD) =
+                mf::decode_as<V>(v.w[i][s], scale);
         }
     }
 }
@@ -417,9 +430,9 @@ template <int HD, class V>
 __device__ __attribute__((always_inline)) inline V value_fragment(const uint16_t *lds, int h, int mt, uint32_t n,
                                                                   uint32_t g) {
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-    const uint16_t *p = lds + (32 * h + 4 * g + n / 4) * kVStride<HD> + 16 * mt + 4 * (n % 4);
+    const uint16_t *p = lds + piece_at<HD>(4 * g + n / 4, 2 * mt + n % 4 / 2) + 4 * (n % 2) + 32 * h * HD;
     const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p));
-    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + 16 * kVStride<HD>));
+    const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + 16 * HD));
     typedef short s16x8 __attribute__((ext_vector_type(8)));
     return __builtin_bit_cast(V, s16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
 }
@@ -686,14 +699,14 @@ __device__ __attribute__((always_inline)) inline uint32_t walk(const Cache &c, c
         __builtin_amdgcn_sched_barrier(0);
         load_codes<HD, TP, false>(c, src.head, src.page_bytes, here, ahead, src.lo, src.hi, at, kc);
         if (ODD) {
-            // NaN blocks of a position, a bit each, behind its row (its lanes are n, n + 16,
+            // NaN blocks of a position, a bit each, behind the rows (its lanes are n, n + 16,
             // n + 32, n + 48); their values are zeros here
 #pragma unroll
             for (uint32_t i = 0; i < kTiles; ++i) {
                 const bool nan = vc.scale[i] == 255;
                 const uint32_t bits = or_over_groups(nan ? 1u << (g * (HD / 4) / 32) : 0u);
                 if (g == 0) {
-                    lds[(16 * i + n) * kVStride<HD> + HD] = uint16_t(bits);
+                    lds[kChunk * HD + 16 * i + n] = uint16_t(bits);
                 }
                 vc.scale[i] = nan ? 127u : vc.scale[i];
 #pragma unroll
@@ -719,8 +732,8 @@ __device__ __attribute__((always_inline)) inline uint32_t walk(const Cache &c, c
                     s[qi][i][j] = M == kHalf && upper ? st[qi][i + kTiles - NT][j] : st[qi][i][j];
                 }
             }
-            softmax_step<HD, M>(s[qi], w.st, qi, w.mine[qi], whole, at0, a.c);
         }
+        softmax_step<HD, M>(s, w.st, w.mine, whole, at0, a.c);
         __builtin_amdgcn_wave_barrier();
         asm volatile("" ::: "memory");
         if (ODD) {
@@ -730,7 +743,7 @@ __device__ __attribute__((always_inline)) inline uint32_t walk(const Cache &c, c
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int32_t p = at0 + 16 * i + j;
-                    const uint32_t bits = lds[(p - int32_t(c0)) * int32_t(kVStride<HD>) + HD];
+                    const uint32_t bits = lds[kChunk * HD + uint32_t(p) - c0];
 #pragma unroll
                     for (int qi = 0; qi < QT; ++qi) {
                         w.nan_blocks[qi] |= p >= w.mine[qi].first && p <= w.mine[qi].last ? bits : 0u;
@@ -761,8 +774,9 @@ __device__ __attribute__((always_inline)) inline void walk_odd(const Cache &c, c
     walk<HD, T, M, TP, true>(c, a, src, chunk, end, kc, vc, here, next, lds, n, g, w);
 }
 
+template <uint32_t W>
 struct ShareScan {
-    uint32_t sum[kWaves];
+    uint32_t sum[W];
     uint32_t block, first;  // the share's first block, and that block's first unit
 };
 
@@ -775,12 +789,12 @@ constexpr int kResident = M == kTwo ? (HD == 64 ? 2 : 1) : HD == 128 || std::is_
 template <int HD, int M>
 union Shared {
     static constexpr uint32_t kOStride = HD + 4;
-    uint16_t v[kWaves][kChunk * kVStride<HD>];
+    uint16_t v[kWaves][kChunk * (HD + 1)];  // rows, and a word per row for its NaN blocks
     struct {
         float o[kWaves][16 * Mode<M>::columns][kOStride];
         float b[kWaves][16 * Mode<M>::columns], l[kWaves][16 * Mode<M>::columns];
     } join;
-    ShareScan scan;
+    ShareScan<kWaves> scan;
 };
 
 // Units [from, to) of a block: the waves take its chunks in turn, and their states are joined.
@@ -916,7 +930,7 @@ __device__ __attribute__((always_inline)) inline void do_block(const Cache &c, c
 // The outputs of a block whose rows see nothing: zeros, or NaN for a sequence that is too long.
 template <int HD, class T>
 __device__ inline void fill_block(const Params &a, uint32_t queries, const Block &k, uint32_t kv_head, T *out) {
-    for (uint32_t u = threadIdx.x; u < queries * (HD / 4); u += kThreads) {
+    for (uint32_t u = threadIdx.x; u < queries * (HD / 4); u += blockDim.x) {
         const uint32_t query = k.query0 + u / (HD / 4), d = 4 * (u % (HD / 4));
         if (query >= k.rows * a.group) {
             break;
@@ -929,73 +943,75 @@ __device__ inline void fill_block(const Params &a, uint32_t queries, const Block
 
 // The part of a share that lies in `block`s, one after the other: `work(k, from, to, place)` does
 // units [from, to) of block k.  Called by every thread of a workgroup.
-template <int HD, class T, class Work>
+template <int HD, class T, uint32_t W, class Work>
 __device__ __attribute__((always_inline)) inline void do_share(const Batch &b, const Params &a, const Plan &plan,
-                                                               ShareScan &scan, T *out, const Work &work) {
+                                                               ShareScan<W> &scan, T *out, const Work &work) {
     const uint32_t share = blockIdx.x, kv_head = blockIdx.y, t = threadIdx.x;
+    uint32_t block, unit = 0, from = 0, to, shares = 0;  // the block, its first unit, the share's units
+    uint64_t total = 0;
     if (plan.single) {
-        // (the blocks with the most positions come last: first of all)
-        const Block k = block_of(b, a, plan.queries, plan.shares - 1 - share);
-        if (k.chunks) {
-            work(k, 0u, units_of(plan, k), -1);
-        } else if (k.exists) {
+        block = plan.shares - 1 - share;  // (the blocks with the most positions come last: first of all)
+        const Block k = block_of(b, a, plan.queries, block);
+        to = units_of(plan, k);
+        if (to == 0 && k.exists) {
             fill_block<HD, T>(a, plan.queries, k, kv_head, out);
         }
-        return;
-    }
-    // every workgroup sums up all blocks' units, and finds where its share begins
-    const uint32_t wave = t / 64, lane = t % 64;
-    const uint32_t per = (plan.blocks + kThreads - 1) / kThreads, mine0 = t * per;
-    uint32_t mine = 0;
-    for (uint32_t i = mine0; i < min(mine0 + per, plan.blocks); ++i) {
-        mine += units_of(plan, block_of(b, a, plan.queries, i));
-    }
-    uint32_t sum = mine;  // of the lanes up to this one
-#pragma unroll
-    for (uint32_t d = 1; d < 64; d <<= 1) {
-        const uint32_t x = __shfl_up(sum, d);
-        sum += lane >= d ? x : 0u;
-    }
-    if (lane == 63) {
-        scan.sum[wave] = sum;
-    }
-    __syncthreads();
-    uint32_t before = sum - mine;
-    uint64_t total = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < kWaves; ++w) {
-        const uint32_t x = scan.sum[w];
-        before += w < wave ? x : 0u;
-        total += x;
-    }
-    const uint32_t shares = uint32_t(min(uint64_t(plan.shares), total));  // a unit each at least
-    if (share >= shares) {
-        return;
-    }
-    const uint32_t from = uint32_t(total * share / shares), to = uint32_t(total * (share + 1) / shares);
-    if (from >= before && from < before + mine) {
-        uint32_t at = before, i = mine0;
-        while (true) {
-            const uint32_t n = units_of(plan, block_of(b, a, plan.queries, i));
-            if (from < at + n) {
-                break;
-            }
-            at += n;
-            ++i;
+    } else {
+        // every workgroup sums up all blocks' units, and finds where its share begins
+        const uint32_t wave = t / 64, lane = t % 64;
+        const uint32_t per = (plan.blocks + W * 64 - 1) / (W * 64), mine0 = t * per;
+        uint32_t mine = 0;
+        for (uint32_t i = mine0; i < min(mine0 + per, plan.blocks); ++i) {
+            mine += units_of(plan, block_of(b, a, plan.queries, i));
         }
-        scan.block = i;
-        scan.first = at;
+        uint32_t sum = mine;  // of the lanes up to this one
+#pragma unroll
+        for (uint32_t d = 1; d < 64; d <<= 1) {
+            const uint32_t x = __shfl_up(sum, d);
+            sum += lane >= d ? x : 0u;
+        }
+        if (lane == 63) {
+            scan.sum[wave] = sum;
+        }
+        __syncthreads();
+        uint32_t before = sum - mine;
+#pragma unroll
+        for (uint32_t w = 0; w < W; ++w) {
+            const uint32_t x = scan.sum[w];
+            before += w < wave ? x : 0u;
+            total += x;
+        }
+        shares = uint32_t(min(uint64_t(plan.shares), total));  // a unit each at least
+        if (share >= shares) {
+            return;
+        }
+        from = uint32_t(total * share / shares);
+        to = uint32_t(total * (share + 1) / shares);
+        if (from >= before && from < before + mine) {
+            uint32_t at = before, i = mine0;
+            while (true) {
+                const uint32_t n = units_of(plan, block_of(b, a, plan.queries, i));
+                if (from < at + n) {
+                    break;
+                }
+                at += n;
+                ++i;
+            }
+            scan.block = i;
+            scan.first = at;
+        }
+        __syncthreads();
+        block = __builtin_amdgcn_readfirstlane(scan.block);
+        unit = __builtin_amdgcn_readfirstlane(scan.first);
+        __syncthreads();
     }
-    __syncthreads();
-    uint32_t block = __builtin_amdgcn_readfirstlane(scan.block), unit = __builtin_amdgcn_readfirstlane(scan.first);
-    __syncthreads();
     while (unit < to) {
         const Block k = block_of(b, a, plan.queries, block);
         const uint32_t units = units_of(plan, k);
         if (units) {
             const uint32_t x = max(from, unit), y = min(to, unit + units);
             const int place = x == unit && y == unit + units ? -1 : x == unit ? 1 : 0;
-            if (place != 0 && kv_head == 0 && t == 0) {
+            if (place != 0 && !plan.single && kv_head == 0 && t == 0) {
                 // the share of a unit u is the last one that begins at u or before
                 const uint64_t last = (uint64_t(unit) + units) * shares - 1;
                 plan.span[block] = make_uint2(share, uint32_t(last / total));
@@ -1012,7 +1028,7 @@ template <int HD, class T, int M, int TP>
 __global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kResident<HD, T, M>))) void
 attention_split_kernel(Cache c, Batch b, Params a, Plan plan, const T *__restrict__ q, T *__restrict__ out) {
     __shared__ __attribute__((aligned(16))) Shared<HD, M> sh;
-    do_share<HD, T>(b, a, plan, sh.scan, out, [&](const Block &k, uint32_t from, uint32_t to, int place) {
+    do_share<HD, T, kWaves>(b, a, plan, sh.scan, out, [&](const Block &k, uint32_t from, uint32_t to, int place) {
         do_block<HD, T, M, TP>(c, b, a, plan, k, blockIdx.y, from, to, place, blockIdx.x, sh, q, out);
     });
 }
@@ -1022,65 +1038,80 @@ attention_split_kernel(Cache c, Batch b, Params a, Plan plan, const T *__restric
 // Each wave converts a tile of 16 positions of the chunk, K to bf16 and V to f16 in LDS, where
 // all four read it; two buffers, so that the next chunk is converted while this one is used,
 // with one barrier a chunk.  A chunk with values outside the f16 path's range is found when it
-// is converted (a flag a wave, beside the buffer) and then converted again, for the bf16 path.
+// is converted (a flag a wave, beside the buffer), and the rest of the walk takes the bf16 path.
 
-template <int HD>
-struct TileShared {
-    union {
-        struct {
-            uint16_t k[2][kChunk * kVStride<HD>], v[2][kChunk * kVStride<HD>];
-        };
-        ShareScan scan;
-    };
-    uint32_t far[2][kWaves];
+// Its waves: 8 with one column tile of queries each, four of which convert K and four V; 4 with
+// two for f32 queries of 64, whose registers leave room for 8 waves a CU either way (4096
+// tokens of 64 heads: 394 against 453 us; heads of 128, 2048 tokens of 20: 8 waves 124 against
+// 151 us in f32, 98 against 99 us in bf16).
+template <int HD, class T>
+struct Tile {
+    static constexpr bool wide = HD == 128 || !std::is_same<T, float>::value;
+    static constexpr uint32_t waves = wide ? 8 : 4, threads = waves * 64;
+    static constexpr int mode = wide ? kOne : kTwo, parts = wide ? 1 : 2;  // parts: what a wave converts
+    static constexpr uint32_t queries = waves * 16 * mode;
+    static constexpr int waves_per_simd = wide && HD == 64 ? 4 : 2;
+    static constexpr uint32_t groups = waves_per_simd * 4 / waves;  // of a CU
 };
 
-// One tile of a chunk's codes (position n, a quarter of the head).
+template <int HD, class T>
+union TileShared {
+    struct {
+        uint16_t k[2][kChunk * HD], v[2][kChunk * HD];
+        uint16_t nan[kChunk], far[2][kTiles];
+    };
+    ShareScan<Tile<HD, T>::waves> scan;
+};
+
+// K's or V's codes of one tile of a chunk (position n, a quarter of the head).
 template <int HD>
 struct TileCodes {
-    uint32_t kw[HD / 32], vw[HD / 32], ks, vs;
+    uint32_t w[HD / 32], scale;
 };
 
 template <int HD, int TP>
 __device__ __attribute__((always_inline)) inline void load_tile(const Cache &c, const Source<TP> &src, uint32_t chunk,
-                                                                uint32_t page, uint32_t wave,
+                                                                uint32_t page, uint32_t index, bool v,
                                                                 const LaneOffsets<HD> &at, TileCodes<HD> &x) {
     using L = Layout<HD>;
-    const uint32_t tile = TP == 1 ? chunk * kTiles + wave : min(max(chunk * kTiles + wave, src.lo / 16), src.hi / 16);
+    const uint32_t tile = TP == 1 ? chunk * kTiles + index : min(max(chunk * kTiles + index, src.lo / 16), src.hi / 16);
     const uint32_t slot = (tile * 16) & ((1u << c.page_shift) - 1);
     const uint8_t *rec = src.head + (page < c.pages ? page : 0u) * src.page_bytes;  // uniform
-    load_words<HD>(rec + L::k_codes(slot) + at.code, x.kw);
-    load_words<HD>(rec + L::v_codes(c.page_shift, slot) + at.code, x.vw);
-    x.ks = (rec + L::k_scales(c.page_shift, slot))[at.scale];
-    x.vs = (rec + L::v_scales(c.page_shift, slot))[at.scale];
+    load_words<HD>(rec + (v ? L::v_codes(c.page_shift, slot) : L::k_codes(slot)) + at.code, x.w);
+    x.scale = (rec + (v ? L::v_scales(c.page_shift, slot) : L::k_scales(c.page_shift, slot)))[at.scale];
 }
 
-// The page of a wave's tile of a chunk.
+// The page of a tile of a chunk.
 template <int TP>
 __device__ __attribute__((always_inline)) inline uint32_t tile_page(const Cache &c, const Source<TP> &src,
-                                                                    uint32_t chunk, uint32_t wave) {
-    const uint32_t tile = TP == 1 ? chunk * kTiles : min(max(chunk * kTiles + wave, src.lo / 16), src.hi / 16);
+                                                                    uint32_t chunk, uint32_t index) {
+    const uint32_t tile = TP == 1 ? chunk * kTiles : min(max(chunk * kTiles + index, src.lo / 16), src.hi / 16);
     return uint32_t(kv4::entry(src.table, tile >> (c.page_shift - 4)));
 }
 
+// The lane's quarter of row n.
 template <int HD, class V>
-__device__ __attribute__((always_inline)) inline void stage_row(uint16_t *row, const uint32_t (&w)[HD / 32],
-                                                                uint32_t scale) {
+__device__ __attribute__((always_inline)) inline void stage_row(uint16_t *rows, uint32_t n, uint32_t g,
+                                                                const uint32_t (&w)[HD / 32], uint32_t scale) {
 #pragma unroll
     for (int s = 0; s < HD / 32; ++s) {
-        *reinterpret_cast<V *>(row + 8 * s) = mf::decode_as<V>(w[s], kv4::scale_of(scale));
+        *reinterpret_cast<V *>(rows + piece_at<HD>(n, g * (HD / 32) + s)) =
+            mf::decode_as<V>(w[s], kv4::scale_of(scale));
     }
 }
 
-template <int HD, class T, int M, int TP>
+template <int HD, class T, int TP>
 __device__ __attribute__((always_inline)) inline void do_tile(const Cache &c, const Batch &b, const Params &a,
                                                               const Plan &plan, const Block &k, uint32_t kv_head,
                                                               uint32_t from, uint32_t to, int place, uint32_t share,
-                                                              TileShared<HD> &sh, const T *q, T *out) {
+                                                              TileShared<HD, T> &sh, const T *q, T *out) {
+    constexpr int M = Tile<HD, T>::mode, KV = Tile<HD, T>::parts;
     constexpr int QT = Mode<M>::columns, NS = HD / 32, QP = kQueryPlanes<T>, PP = kWeightPlanes<T>;
     uint32_t t = threadIdx.x;
     asm volatile("" : "+v"(t));  // (as in do_block)
     const uint32_t wave = __builtin_amdgcn_readfirstlane(t / 64), lane = t % 64, n = lane % 16, g = lane / 16;
+    const uint32_t index = wave % kTiles;  // of the tile that the wave converts
+    const auto is_v = [&](int part) __attribute__((always_inline)) { return KV == 2 ? part == 1 : wave >= kTiles; };
     Source<TP> src;
     src.table = b.table + size_t(k.sequence) * b.stride;
     src.page_bytes = size_t(c.kv_heads) * c.record;
@@ -1123,126 +1154,159 @@ __device__ __attribute__((always_inline)) inline void do_tile(const Cache &c, co
         }
     }
 
-    TileCodes<HD> x;
-    // positions of the tile outside lo..hi, and pages that are not there
+    TileCodes<HD> x[KV];
+    const auto load = [&](uint32_t chunk, uint32_t page) __attribute__((always_inline)) {
+#pragma unroll
+        for (int part = 0; part < KV; ++part) {
+            load_tile<HD, TP>(c, src, chunk, page, index, is_v(part), at, x[part]);
+        }
+    };
+    // a page that is not there: keys read as NaN; values outside lo..hi are zeros
     const auto trim = [&](uint32_t chunk, uint32_t page) __attribute__((always_inline)) {
-        const uint32_t p = chunk * kChunk + 16 * wave + n;
+        const uint32_t p = chunk * kChunk + 16 * index + n;
         const bool inside = chunk * kChunk >= src.lo && chunk * kChunk + kChunk - 1 <= src.hi;
         if (!inside || page >= c.pages) {
             const bool zero = p < src.lo || p > src.hi || page >= c.pages;
-            x.ks = page >= c.pages ? 255u : x.ks;
-            x.vs = zero ? 127u : x.vs;
 #pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                x.vw[s] = zero ? 0u : x.vw[s];
+            for (int part = 0; part < KV; ++part) {
+                if (!is_v(part)) {
+                    x[part].scale = page >= c.pages ? 255u : x[part].scale;
+                    continue;
+                }
+                x[part].scale = zero ? 127u : x[part].scale;
+#pragma unroll
+                for (int s = 0; s < NS; ++s) {
+                    x[part].w[s] = zero ? 0u : x[part].w[s];
+                }
             }
         }
     };
-    const auto stage = [&](uint32_t chunk, uint32_t page) __attribute__((always_inline)) {
+    const auto stage = [&](uint32_t buffer, uint32_t chunk, uint32_t page) __attribute__((always_inline)) {
         trim(chunk, page);
-        const uint32_t buf = chunk % 2, row = (16 * wave + n) * kVStride<HD> + g * (HD / 4);
-        stage_row<HD, bf16x8>(sh.k[buf] + row, x.kw, x.ks);
-        stage_row<HD, f16x8>(sh.v[buf] + row, x.vw, x.vs);
-        const bool far = __any(x.vs - kF16First > kF16Last - kF16First);
-        if (lane == 0) {
-            sh.far[buf][wave] = far ? 1u : 0u;
+        const uint32_t buf = buffer % 2;
+#pragma unroll
+        for (int part = 0; part < KV; ++part) {
+            if (!is_v(part)) {
+                stage_row<HD, bf16x8>(sh.k[buf] + 16 * index * HD, n, g, x[part].w, x[part].scale);
+                continue;
+            }
+            stage_row<HD, f16x8>(sh.v[buf] + 16 * index * HD, n, g, x[part].w, x[part].scale);
+            const bool far = __any(x[part].scale - kF16First > kF16Last - kF16First);
+            if (lane == 0) {
+                sh.far[buf][index] = far ? 1u : 0u;
+            }
         }
     };
-    uint32_t page = tile_page<TP>(c, src, first, wave);
-    uint32_t next = tile_page<TP>(c, src, min(first + 1, end - 1), wave);
-    load_tile<HD, TP>(c, src, first, page, wave, at, x);
-    stage(first, page);
+    uint32_t page = tile_page<TP>(c, src, first, index);
+    uint32_t next = tile_page<TP>(c, src, min(first + 1, end - 1), index);
+    load(first, page);
+    stage(first, first, page);
     page = next;
-    next = tile_page<TP>(c, src, min(first + 2, end - 1), wave);
-    load_tile<HD, TP>(c, src, min(first + 1, end - 1), page, wave, at, x);
+    next = tile_page<TP>(c, src, min(first + 2, end - 1), index);
+    load(min(first + 1, end - 1), page);
     __syncthreads();
 
-#pragma unroll 1
-    for (uint32_t chunk = first; chunk < end; ++chunk) {
-        const uint32_t buf = chunk % 2;
-        const int32_t c0 = int32_t(chunk * kChunk);
-        const bool far = (sh.far[buf][0] | sh.far[buf][1] | sh.far[buf][2] | sh.far[buf][3]) != 0;
-        // (every thread sees the same flags: all of them take the same way, with its barriers)
-        const bool odd = __builtin_amdgcn_readfirstlane(uint32_t(far)) != 0;
-        const bool needed = any && c0 <= p1 && c0 + int32_t(kChunk) > first_min;
-        const bool whole = c0 >= first_max && c0 + int32_t(kChunk) - 1 <= p0;
-        f32x4 s[QT][kTiles];
-        if (needed) {
-            const uint16_t *const ks = sh.k[buf] + n * kVStride<HD> + g * (HD / 4);
+    const auto scores = [&](uint32_t buf, f32x4 (&s)[QT][kTiles]) __attribute__((always_inline)) {
 #pragma unroll
-            for (int step = 0; step < NS; ++step) {
-                bf16x8 kf[kTiles];
+        for (int step = 0; step < NS; ++step) {
+            const uint16_t *const ks = sh.k[buf] + piece_at<HD>(n, g * (HD / 32) + step);
+            bf16x8 kf[kTiles];
+#pragma unroll
+            for (uint32_t i = 0; i < kTiles; ++i) {
+                kf[i] = *reinterpret_cast<const bf16x8 *>(ks + 16 * i * HD);
+            }
+#pragma unroll
+            for (int p = QP - 1; p >= 0; --p) {
 #pragma unroll
                 for (uint32_t i = 0; i < kTiles; ++i) {
-                    kf[i] = *reinterpret_cast<const bf16x8 *>(ks + 16 * i * kVStride<HD> + 8 * step);
-                }
 #pragma unroll
-                for (int p = QP - 1; p >= 0; --p) {
-#pragma unroll
-                    for (uint32_t i = 0; i < kTiles; ++i) {
-#pragma unroll
-                        for (int qi = 0; qi < QT; ++qi) {
-                            s[qi][i] = mf::mfma(kf[i], qf[qi][step][p],
-                                                step == 0 && p == QP - 1 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[qi][i]);
-                        }
+                    for (int qi = 0; qi < QT; ++qi) {
+                        s[qi][i] = mf::mfma(kf[i], qf[qi][step][p],
+                                            step == 0 && p == QP - 1 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[qi][i]);
                     }
                 }
             }
         }
-        // the next chunk into the other buffer, whose readers are behind the last barrier
-        if (chunk + 1 < end) {
-            stage(chunk + 1, page);
-            page = next;
-            next = tile_page<TP>(c, src, min(chunk + 3, end - 1), wave);
-            load_tile<HD, TP>(c, src, min(chunk + 2, end - 1), page, wave, at, x);
+    };
+    const auto needed = [&](uint32_t chunk) __attribute__((always_inline)) {
+        const int32_t c0 = int32_t(chunk * kChunk);
+        return any && c0 <= p1 && c0 + int32_t(kChunk) > first_min;
+    };
+    const auto soften = [&](uint32_t chunk, f32x4 (&s)[QT][kTiles]) __attribute__((always_inline)) {
+        const int32_t c0 = int32_t(chunk * kChunk);
+        const bool whole = c0 >= first_max && c0 + int32_t(kChunk) - 1 <= p0;
+        softmax_step<HD, M>(s, st, mine, whole, c0 + int32_t(4 * g), a.c);
+    };
+    uint32_t chunk = first;
+#pragma unroll 1
+    for (; chunk < end; ++chunk) {
+        const uint32_t buf = chunk % 2;
+        // every thread sees the same flags, so all of them go the same way
+        const uint32_t far = uint32_t(sh.far[buf][0] | sh.far[buf][1]) | uint32_t(sh.far[buf][2] | sh.far[buf][3]);
+        if (__builtin_amdgcn_readfirstlane(far)) {
+            break;
         }
-        if (needed) {
+        f32x4 s[QT][kTiles];
+        if (needed(chunk)) {
+            scores(buf, s);
+        }
+        // the next chunk into the other buffer, whose readers are behind the last barrier (at the
+        // end the last one again, which nobody reads)
+        stage(chunk + 1, min(chunk + 1, end - 1), page);
+        page = next;
+        next = tile_page<TP>(c, src, min(chunk + 3, end - 1), index);
+        load(min(chunk + 2, end - 1), page);
+        if (needed(chunk)) {
+            soften(chunk, s);
+            weigh_values<HD, f16x8, PP, M>(sh.v[buf], s, st, n, g);
+        }
+        __syncthreads();
+    }
+    // From a chunk with values outside the f16 path's range on: V as bf16, its NaN blocks as
+    // zeros and counted apart; one buffer.
+#pragma unroll 1
+    for (; chunk < end; ++chunk) {
+        const uint32_t here = tile_page<TP>(c, src, chunk, index);
+        load(chunk, here);
+        trim(chunk, here);
+        __syncthreads();
 #pragma unroll
-            for (int qi = 0; qi < QT; ++qi) {
-                softmax_step<HD, M>(s[qi], st, qi, mine[qi], whole, c0 + int32_t(4 * g), a.c);
+        for (int part = 0; part < KV; ++part) {
+            if (!is_v(part)) {
+                stage_row<HD, bf16x8>(sh.k[0] + 16 * index * HD, n, g, x[part].w, x[part].scale);
+                continue;
             }
-            if (!odd) {
-                weigh_values<HD, f16x8, PP, M>(sh.v[buf], s, st, n, g);
-            }
-        }
-        if (odd) {
-            // V again, as bf16, its NaN blocks as zeros and a bit each behind their row
-            __syncthreads();
-            const uint32_t here = tile_page<TP>(c, src, chunk, wave);
-            const TileCodes<HD> keep = x;
-            load_tile<HD, TP>(c, src, chunk, here, wave, at, x);
-            trim(chunk, here);
-            const bool nan = x.vs == 255;
+            const bool nan = x[part].scale == 255;
             const uint32_t bits = or_over_groups(nan ? 1u << (g * (HD / 4) / 32) : 0u);
-            uint16_t *const row = sh.v[buf] + (16 * wave + n) * kVStride<HD>;
-            if (g == 0) {
-                row[HD] = uint16_t(bits);
-            }
-            x.vs = nan ? 127u : x.vs;
+            x[part].scale = nan ? 127u : x[part].scale;
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
-                x.vw[i] = nan ? 0u : x.vw[i];
+                x[part].w[i] = nan ? 0u : x[part].w[i];
             }
-            stage_row<HD, bf16x8>(row + g * (HD / 4), x.vw, x.vs);
-            x = keep;
-            __syncthreads();
-            if (needed) {
-                weigh_values_odd<HD, M>(sh.v[buf], s, st, n, g);
-#pragma unroll
-                for (uint32_t i = 0; i < kTiles; ++i) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int32_t local = int32_t(16 * i + 4 * g) + j, p = c0 + local;
-                        const uint32_t nans = sh.v[buf][local * int32_t(kVStride<HD>) + HD];
-#pragma unroll
-                        for (int qi = 0; qi < QT; ++qi) {
-                            nan_blocks[qi] |= p >= mine[qi].first && p <= mine[qi].last ? nans : 0u;
-                        }
-                    }
-                }
+            stage_row<HD, bf16x8>(sh.v[0] + 16 * index * HD, n, g, x[part].w, x[part].scale);
+            if (g == 0) {
+                sh.nan[16 * index + n] = uint16_t(bits);
             }
         }
         __syncthreads();
+        if (needed(chunk)) {
+            f32x4 s[QT][kTiles];
+            scores(0, s);
+            soften(chunk, s);
+            weigh_values_odd<HD, M>(sh.v[0], s, st, n, g);
+#pragma unroll
+            for (uint32_t i = 0; i < kTiles; ++i) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int32_t local = int32_t(16 * i + 4 * g) + j, p = int32_t(chunk * kChunk) + local;
+                    const uint32_t nans = sh.nan[local];
+#pragma unroll
+                    for (int qi = 0; qi < QT; ++qi) {
+                        nan_blocks[qi] |= p >= mine[qi].first && p <= mine[qi].last ? nans : 0u;
+                    }
+                }
+            }
+        }
     }
 
 #pragma unroll
@@ -1277,31 +1341,30 @@ __device__ __attribute__((always_inline)) inline void do_tile(const Cache &c, co
     }
 }
 
-// Workgroups of a CU.
-template <int HD, class T, int M>
-constexpr int kTileResident = HD == 128 && std::is_same<T, float>::value ? 1 : 2;
-
-template <int HD, class T, int M, int TP>
-__global__ __launch_bounds__(kThreads) __attribute__((amdgpu_waves_per_eu(kTileResident<HD, T, M>))) void
+template <int HD, class T, int TP>
+__global__ __launch_bounds__((Tile<HD, T>::threads)) __attribute__((amdgpu_waves_per_eu(Tile<HD, T>::waves_per_simd))) void
 attention_tile_kernel(Cache c, Batch b, Params a, Plan plan, const T *__restrict__ q, T *__restrict__ out) {
-    __shared__ __attribute__((aligned(16))) TileShared<HD> sh;
-    do_share<HD, T>(b, a, plan, sh.scan, out, [&](const Block &k, uint32_t from, uint32_t to, int place) {
-        do_tile<HD, T, M, TP>(c, b, a, plan, k, blockIdx.y, from, to, place, blockIdx.x, sh, q, out);
-    });
+    __shared__ __attribute__((aligned(16))) TileShared<HD, T> sh;
+    do_share<HD, T, Tile<HD, T>::waves>(
+        b, a, plan, sh.scan, out, [&](const Block &k, uint32_t from, uint32_t to, int place) {
+            do_tile<HD, T, TP>(c, b, a, plan, k, blockIdx.y, from, to, place, blockIdx.x, sh, q, out);
+        });
 }
 
 // ---- the parts of a block joined ---------------------------------------------------------------
 
-// W waves per row and head (4 where a block may have many parts, else 1): each takes a share of
-// the parts, 64 / (HD / 4) at a time.
-template <int HD, class T, int W>
+// W waves per row and head, P parts at a time each (HD / 4 lanes a part): 4 waves where few
+// rows may have many parts; one where rows are few; else only the lanes of one part (P = 1),
+// which takes fewer waves for what is mostly waiting (512 tokens of 64 heads at 2048: 61 against
+// 69 us with the attention, 4 tokens of 8 sequences at 16384: 35 against 33).
+template <int HD, class T, int W, int P>
 __global__ __launch_bounds__(kThreads) void attention_join_kernel(Cache c, Batch b, Params a, Plan plan,
                                                                   T *__restrict__ out) {
-    constexpr uint32_t kLanes = HD / 4, kParts = 64 / kLanes;  // lanes of an output, parts of a wave at a time
+    constexpr uint32_t kLanes = HD / 4, kSpan = P * kLanes, kRows = 64 / kSpan;  // rows (and heads) of a wave
     __shared__ float part_l[kWaves];
     __shared__ f32x4 part_o[kWaves][kLanes];
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % 64;
-    const uint32_t at = blockIdx.x * (kWaves / W) + wave / W, turn = wave % W;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), lane = threadIdx.x % kSpan;
+    const uint32_t at = (blockIdx.x * (kWaves / W) + wave / W) * kRows + threadIdx.x % 64 / kSpan, turn = wave % W;
     const uint32_t row = at / a.heads, head = at % a.heads, kv_head = head / a.group;
     const uint32_t part = lane / kLanes, d = 4 * (lane % kLanes);
     T *const dst = out + (size_t(row) * a.heads + head) * HD + d;
@@ -1331,16 +1394,16 @@ __global__ __launch_bounds__(kThreads) void attention_join_kernel(Cache c, Batch
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     float top = -INFINITY, l = 0.0f;
     if (parts > 1) {
-        for (uint32_t i = lane; i < parts; i += 64) {
+        for (uint32_t i = lane; i < parts; i += kSpan) {
             top = fmaxf(top, plan.bl[place(i)].x);
         }
 #pragma unroll
-        for (int x = 32; x >= 1; x >>= 1) {
+        for (int x = kSpan / 2; x >= 1; x >>= 1) {
             top = fmaxf(top, __shfl_xor(top, x));
         }
         const float offset = top == -INFINITY ? 0.0f : top;
 #pragma unroll 4
-        for (uint32_t i = turn * kParts + part; i < parts; i += W * kParts) {
+        for (uint32_t i = turn * P + part; i < parts; i += W * P) {
             const float2 s = plan.bl[place(i)];
             const f32x4 x = *reinterpret_cast<const f32x4 *>(plan.o + place(i) * HD + d);
             const float f = __builtin_amdgcn_exp2f(s.x - offset);
@@ -1351,7 +1414,7 @@ __global__ __launch_bounds__(kThreads) void attention_join_kernel(Cache c, Batch
             }
         }
 #pragma unroll
-        for (uint32_t x = kLanes; x < 64; x <<= 1) {
+        for (uint32_t x = kLanes; x < kSpan; x <<= 1) {
             l += __shfl_xor(l, x);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -1427,15 +1490,18 @@ Cut cut_of(const ttl_kv4_cache *cache, const ttl_kv4_batch *batch, const ttl_kv4
     const uint64_t mean = queries / batch->sequences;
     Plan &p = cut.plan;
     cut.tile = batch->starts && mean >= kTileFrom;
-    uint64_t slots;
+    uint64_t slots = 0;
     if (cut.tile) {
-        // four column tiles a wave read K and V from LDS half as often as two do; two leave more
-        // workgroups
-        const bool four = false && !f32 && cache->head_dim == 64 && queries / 256 * cache->kv_heads >= 2 * kCus;
-        cut.mode = four ? kFour : kTwo;
-        p.queries = kWaves * 16 * uint32_t(cut.mode);
+        const auto take = [&](auto tile) {
+            p.queries = decltype(tile)::queries;
+            slots = kCus * decltype(tile)::groups;
+        };
+        if (cache->head_dim == 64) {
+            f32 ? take(Tile<64, float>()) : take(Tile<64, __bf16>());
+        } else {
+            f32 ? take(Tile<128, float>()) : take(Tile<128, __bf16>());
+        }
         p.unit = 1;
-        slots = kCus * (cache->head_dim == 128 && f32 ? 1 : 2);
     } else {
         cut.mode = mean > 16 ? kTwo : mean > 8 ? kOne : kHalf;
         p.queries = cut.mode == kTwo ? 32 : cut.mode == kOne ? 16 : 8;
@@ -1453,9 +1519,11 @@ Cut cut_of(const ttl_kv4_cache *cache, const ttl_kv4_batch *batch, const ttl_kv4
     }
     const uint32_t chunks = longest / kChunk + (attention->window ? 2 : 1);  // any alignment
     const uint64_t units = (chunks + p.unit - 1) / p.unit;
-    // With enough blocks (or so many that finding a share would take long) a workgroup takes a
-    // block whole.
-    p.single = units == 1 || (cut.tile && uint64_t(p.blocks) * cache->kv_heads >= 2 * slots) || p.blocks > 1u << 16;
+    // A workgroup takes a block whole where blocks are enough (1024 tokens at 2048: 61 against 87
+    // us), or short enough for half as many (4 x 128 tokens at 1024: 35 against 47 us; but 512 at
+    // 8192: 198 against 137), or so many that finding a share would take long.
+    const uint64_t all = uint64_t(p.blocks) * cache->kv_heads;
+    p.single = units == 1 || (cut.tile && (all >= slots || (2 * all >= slots && units <= 24))) || p.blocks > 1u << 16;
     if (p.single) {
         p.shares = p.blocks;
         return cut;
@@ -1490,7 +1558,7 @@ int run_attention(ttl_ctx *ctx, const ttl_kv4_cache *cache, const ttl_kv4_batch 
     TTL_REQUIRE(cut.workspace == 0 || (uintptr_t(workspace) & 255) == 0, TTL_ERR_INVALID,
                 "%s: the workspace must be 256-byte aligned", what);
     const uint64_t groups = uint64_t(cut.plan.shares) * cache->kv_heads;
-    TTL_REQUIRE(groups * kThreads <= 0xffffffffu && uint64_t(batch->tokens) * attention->heads <= 0x7fffffffu, TTL_ERR_SHAPE,
+    TTL_REQUIRE(groups * 2 * kThreads <= 0xffffffffu && uint64_t(batch->tokens) * attention->heads <= 0x7fffffffu, TTL_ERR_SHAPE,
                 "%s: %u tokens of %u heads are too many for one call", what, batch->tokens, attention->heads);
     TTL_HIP(hipSetDevice(ctx->device));
     const Cache c = kv4::view(cache);
@@ -1527,22 +1595,12 @@ int run_attention(ttl_ctx *ctx, const ttl_kv4_cache *cache, const ttl_kv4_batch 
                 attention_split_kernel<HD, T, M, 4><<<grid, kThreads, 0, ctx->stream>>>(c, b, a, p, qt, ot);
             }
         };
-        const auto tile = [&](auto mode) {
-            constexpr int M = decltype(mode)::value;
-            if (big) {
-                attention_tile_kernel<HD, T, M, 1><<<grid, kThreads, 0, ctx->stream>>>(c, b, a, p, qt, ot);
-            } else {
-                attention_tile_kernel<HD, T, M, 4><<<grid, kThreads, 0, ctx->stream>>>(c, b, a, p, qt, ot);
-            }
-        };
         if (cut.tile) {
-            if constexpr (HD == 64 && !std::is_same<T, float>::value) {
-                if (cut.mode == kFour) {
-                    tile(std::integral_constant<int, kFour>());
-                }
-            }
-            if (cut.mode == kTwo) {
-                tile(std::integral_constant<int, kTwo>());
+            constexpr uint32_t threads = Tile<HD, T>::threads;
+            if (big) {
+                attention_tile_kernel<HD, T, 1><<<grid, threads, 0, ctx->stream>>>(c, b, a, p, qt, ot);
+            } else {
+                attention_tile_kernel<HD, T, 4><<<grid, threads, 0, ctx->stream>>>(c, b, a, p, qt, ot);
             }
         } else if (cut.mode == kHalf) {
             split(std::integral_constant<int, kHalf>());
@@ -1553,11 +1611,15 @@ int run_attention(ttl_ctx *ctx, const ttl_kv4_cache *cache, const ttl_kv4_batch 
         }
         if (!p.single) {
             const size_t rows = size_t(b.tokens) * a.heads;
+            constexpr int P = 256 / HD;
             if (cut.most_parts > 16 && rows <= 1024) {
-                attention_join_kernel<HD, T, 4><<<uint32_t(rows), kThreads, 0, ctx->stream>>>(c, b, a, p, ot);
+                attention_join_kernel<HD, T, 4, P><<<uint32_t(rows), kThreads, 0, ctx->stream>>>(c, b, a, p, ot);
+            } else if (rows <= 4096) {
+                attention_join_kernel<HD, T, 1, P><<<ttl::blocks_for(rows, kWaves), kThreads, 0, ctx->stream>>>(
+                    c, b, a, p, ot);
             } else {
-                attention_join_kernel<HD, T, 1><<<ttl::blocks_for(rows, kWaves), kThreads, 0, ctx->stream>>>(c, b, a, p,
-                                                                                                     ot);
+                attention_join_kernel<HD, T, 1, 1><<<ttl::blocks_for(rows, kWaves * P), kThreads, 0, ctx->stream>>>(
+                    c, b, a, p, ot);
             }
         }
     };
