@@ -133,6 +133,11 @@ def attention(q, k, v, positions, first, window, scale, sinks):
             p = np.where(seen, np.exp(s - m), 0.0)
             den = p.sum(1, keepdims=True) + (np.exp(float(sinks[h]) - m) if sinks is not None else 0.0)
             vis = seen.any(1)
+            if np.isfinite(v[:, g]).all():  # (an unseen value times a weight of 0 is 0)
+                n = np.where(vis[:, None], den, 1.0)
+                out[:, h], mag[:, h] = p @ v[:, g] / n, p @ np.abs(v[:, g]) / n
+                vsum[:, h] = seen @ np.abs(v[:, g])
+                continue
             for r in np.nonzero(vis)[0]:
                 w, vv = p[r][seen[r]], v[:, g][seen[r]]
                 out[r, h] = w @ vv / den[r]

@@ -722,3 +722,128 @@ def test_results_repeat(dev, held, prefill):
     q = rng.standard_normal((12 if prefill else 2, 64, 64)).astype(np.float32)
     a, b = (run_attention(dev, held, pb, pool, table, lengths, news, q, 64, F32, 0, 0.125, None) for _ in range(2))
     assert np.array_equal(a, b)
+
+
+# ---- the ways a call is cut -------------------------------------------------------------------------
+#
+# By the queries that a sequence has on average for a key/value head: 8 and fewer, 16, 32, more;
+# blocks divided among workgroups or taken whole; outputs joined by 4 waves, one, or part of one.
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,page,news", [
+    (16, 2, 64, 16, [1, 1, 1, 0, 1]), (16, 2, 64, 64, [1, 3, 2, 0, 1]), (16, 2, 64, 16, [3, 1, 6, 2, 4]),
+    (16, 2, 64, 64, [7, 1, 9, 0, 8]), (20, 4, 128, 32, [1, 1, 2, 0, 1]), (20, 4, 128, 128, [2, 1, 4, 1, 3]),
+    (20, 4, 128, 16, [6, 1, 9, 2, 5]), (20, 4, 128, 64, [21, 1, 30, 0, 14])])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("window", [0, 100])
+def test_prefill_few_tokens(dev, held, heads, kv_heads, hd, page, news, dtype, window):
+    rng = np.random.default_rng(sum(news) + window)
+    lengths = [6000, 1, 130, 0, 2501]
+    pages = sum(-(-n // page) for n in lengths) + 1
+    pool = R.Pool(pages, kv_heads, hd, page).randomise(rng)
+    table = R.tables(rng, lengths, page, pages)
+    q, qb = to_dtype(rng.standard_normal((sum(news) + 3, heads, hd)) * 1.5, dtype)
+    sinks = rng.standard_normal(heads).astype(np.float32)
+    scale = float(np.float32(hd ** -0.5))
+    got = run_attention(dev, held, held.up(pool.bytes), pool, table, lengths, news, qb, heads, dtype, window, scale,
+                        sinks)
+    check_attention(got, q, pool, table, lengths, news, heads, dtype, window, scale, sinks)
+    fill = R.from_bf16(np.uint16([0x5a5a])) if dtype == BF16 else np.uint32([0x5a5a5a5a]).view(np.float32)
+    assert (got[sum(news):] == float(fill[0])).all()
+
+
+@pytest.mark.parametrize("group,kv_heads,news_to", [(8, 1, 0), (20, 1, 0), (4, 2, 2), (8, 1, 5), (8, 2, 24)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_many_sequences(dev, held, group, kv_heads, news_to, dtype):
+    """More blocks than a workgroup has threads, of very different lengths, some without rows."""
+    rng = np.random.default_rng(31 + group + news_to)
+    count, heads, page = 700, group * kv_heads, 16
+    lengths = rng.integers(0, 60, count)
+    lengths[rng.integers(0, count, 6)] = [3000, 900, 1, 257, 64, 2000]
+    lengths[0], lengths[-1] = 0, 500
+    news = rng.integers(0, news_to + 1, count) if news_to else None
+    pages = int(sum(-(-n // page) for n in lengths)) + 1
+    pool = R.Pool(pages, kv_heads, 64, page).randomise(rng)
+    table = R.tables(rng, lengths, page, pages)
+    if news_to:
+        # (no more new tokens than a sequence holds, or none at all of it: idle rows)
+        news = np.where(lengths > 0, np.minimum(news, lengths), news)
+    each = news if news_to else np.ones(count, np.int64)
+    q, qb = to_dtype(rng.standard_normal((int(each.sum()), heads, 64)), dtype)
+    got = run_attention(dev, held, held.up(pool.bytes), pool, table, lengths, news, qb, heads, dtype, 0, 0.125, None)
+    check_attention(got, q, pool, table, lengths, each, heads, dtype, 0, 0.125, None)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,news,lengths,window", [
+    (64, 8, 64, [1030], [1030], 0),             # blocks enough to be taken whole
+    (64, 8, 64, [700, 1, 0, 350], [5000, 1, 9, 901], 100),
+    (64, 8, 64, [300, 290], [900, 290], 0),     # short ones, half as many
+    (64, 8, 64, [300], [3001], 0),              # divided
+    (20, 4, 128, [900, 130], [901, 600], 0),
+    (20, 4, 128, [150, 3], [2000, 700], 0),
+])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_prompts(dev, held, heads, kv_heads, hd, news, lengths, window, dtype):
+    rng = np.random.default_rng(sum(news))
+    page = 64
+    pages = sum(-(-n // page) for n in lengths)
+    pool = R.Pool(pages, kv_heads, hd, page).randomise(rng)
+    table = R.tables(rng, lengths, page, pages)
+    q, qb = to_dtype(rng.standard_normal((sum(news), heads, hd)) * 1.5, dtype)
+    sinks = rng.standard_normal(heads).astype(np.float32)
+    scale = float(np.float32(hd ** -0.5))
+    got = run_attention(dev, held, held.up(pool.bytes), pool, table, lengths, news, qb, heads, dtype, window, scale,
+                        sinks)
+    check_attention(got, q, pool, table, lengths, news, heads, dtype, window, scale, sinks)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,news", [(20, 4, 128, None), (20, 4, 128, [2, 3]), (20, 4, 128, [90, 40]),
+                                                    (40, 4, 64, None), (16, 2, 64, [2, 5]), (16, 2, 64, [90, 40])])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_values_outside_the_half_range(dev, held, heads, kv_heads, hd, news, dtype):
+    """Single blocks of V with scale bytes below 104 or above 140, from the middle of a sequence on."""
+    rng = np.random.default_rng(41)
+    page, lengths = 32, [1500, 300]
+    pool = R.Pool(64, kv_heads, hd, page).randomise(rng)
+    table = R.tables(rng, lengths, page, 64)
+    for s, p, d, f in [(0, 800, 3, 2.0 ** 30), (0, 801, hd - 1, 2.0 ** -60), (0, 1300, 40, 2.0 ** 20), (1, 10, 0, 2.0 ** 100),
+                       (1, 299, 33, 2.0 ** 19)]:
+        k, v = pool.get(table[s], np.array([p]))
+        v[0, :, d // 32 * 32:d // 32 * 32 + 32] *= f
+        pool.put(table[s], p, k[0], v[0])
+    n = sum(news) if news else 2
+    q, qb = to_dtype(rng.standard_normal((n, heads, hd)), dtype)
+    got = run_attention(dev, held, held.up(pool.bytes), pool, table, lengths, news, qb, heads, dtype, 0, 0.125, None)
+    check_attention(got, q, pool, table, lengths, news or [1, 1], heads, dtype, 0, 0.125, None)
+
+
+@pytest.mark.parametrize("news", [[3, 2], [40, 1], [200, 60]])
+def test_captured_prompts(dev, held, news):
+    """A prompt pass captured once, replayed for other lengths and another division of its rows,
+    with eager work between the replays."""
+    rng = np.random.default_rng(sum(news))
+    heads, kv, page, seqs, tokens = 64, 8, 64, 2, sum(news)
+    stride = 40
+    table = rng.permutation(128)[:seqs * stride].reshape(seqs, stride).astype(np.int32)
+    pool = R.Pool(128, kv, 64, page).randomise(rng)
+    pb, tb, lb, sb = held.up(pool.bytes), held.up(table), held.up(np.int32([1, 1])), held.up(cumulative(news))
+    cache = T.kv4_cache(pb, 128, kv, 64, page)
+    batch = T.kv4_batch(seqs, tokens, tb, stride, lb, sb, None, page)
+    att = T.kv4_attention(heads, BF16, 0, 0.125, None)
+    need = dev.attention_kv4_workspace_bytes(cache, batch, att)
+    q = held.new(tokens * heads * 64 * 2)
+    outs = [held.new(tokens * heads * 64 * 2, 0x5a) for _ in range(2)]
+    spaces = [held.new(max(need, 16), 0xff) for _ in range(2)]
+    graph = dev.capture(lambda: dev.attention_prefill_kv4(cache, batch, att, q, outs[1], spaces[1], need))
+    for step, (lengths, split) in enumerate([([2000, 100], news), ([2400, 900], news[::-1]), ([tokens, 0], [tokens, 0]),
+                                             ([3, 2500], [1, tokens - 1]), ([2000, 100], news)]):
+        lb.upload(np.int32(lengths))
+        sb.upload(cumulative(split))
+        q.upload(to_dtype(rng.standard_normal((tokens, heads, 64)), BF16)[1])
+        dev.attention_prefill_kv4(cache, batch, att, q, outs[0], spaces[0], need)
+        dev.sync()
+        graph.launch()
+        dev.sync()
+        a, b = (o.download(np.uint16, tokens * heads * 64) for o in outs)
+        assert np.array_equal(a, b) and (a != 0x5a5a).any(), step
+    graph.free()

@@ -781,8 +781,8 @@ struct ShareScan {
 };
 
 // Workgroups of a CU (waves of a SIMD).  More would fit on 128 registers with M kHalf, and were
-// slower: 4 instead of 3 for bf16 queries 51.8 against 49.8 us (64 ragged sequences up to
-// 8192), 3 instead of 2 for f32 79.9 against 74.1 us (128 at 4096).
+// slower: 4 instead of 3 for bf16 queries 51.7 against 49.2 us (64 ragged sequences up to
+// 8192), 3 instead of 2 for f32 78.1 against 72.6 us (128 at 4096).
 template <int HD, class T, int M>
 constexpr int kResident = M == kTwo ? (HD == 64 ? 2 : 1) : HD == 128 || std::is_same<T, float>::value ? 2 : 3;
 
