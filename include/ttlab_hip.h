@@ -640,15 +640,19 @@ size_t ttl_attention_kv4_workspace_bytes(const ttl_kv4_cache *cache, const ttl_k
  * position, the sink in the maximum and the denominator only (model.cpp:270-281): q_dev and
  * out_dev [sequences][heads][head_dim] of attention->dtype, 16-byte aligned.  A query with a
  * value that is not finite gives NaN, as does one that sees a NaN block; masked positions
- * have no influence whatever they hold.  Products, sums and the softmax are f32.
+ * have no influence whatever they hold.  Scores are f32 sums of exact products (f32 queries
+ * as three bf16 planes, 24 bits), their maxima, the exponentials' sums and the outputs f32.  The
+ * weights go into the product with V as f16 for a bf16 output (2^-11 of a weight) and as two
+ * f16 planes for an f32 one (2^-22; weights far below the largest seen so far lose at most 2^-32
+ * of that one).  Results depend on nothing but the call: the same one gives the same bits.
  * workspace_dev is caller-owned, 256-byte aligned, of the size above; calls sharing one must
  * not overlap. */
 int ttl_attention_decode_kv4(ttl_ctx *ctx, const ttl_kv4_cache *cache, const ttl_kv4_batch *batch,
                              const ttl_kv4_attention *attention, const void *q_dev, void *out_dev,
                              void *workspace_dev, size_t workspace_bytes);
 /* The same for runs of tokens (batch->starts given), prompt passes of several sequences in one
- * call: q_dev and out_dev [tokens][heads][head_dim].  The cache must hold the rows' own keys
- * and values already. */
+ * call: q_dev and out_dev [tokens][heads][head_dim], tokens x heads at most 2^31 - 1.  The cache
+ * must hold the rows' own keys and values already. */
 int ttl_attention_prefill_kv4(ttl_ctx *ctx, const ttl_kv4_cache *cache, const ttl_kv4_batch *batch,
                               const ttl_kv4_attention *attention, const void *q_dev, void *out_dev,
                               void *workspace_dev, size_t workspace_bytes);

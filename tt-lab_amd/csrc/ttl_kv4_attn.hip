@@ -1378,8 +1378,9 @@ __global__ __launch_bounds__(kThreads) void attention_join_kernel(Cache c, Batch
             const uint32_t block = b.starts ? uint32_t(uint64_t(row0) * a.group / plan.queries) + r.sequence
                                             : r.sequence * ((a.group + plan.queries - 1) / plan.queries);
             const uint2 span = plan.span[block + query / plan.queries];
-            first = span.x;
-            parts = span.y - span.x + 1;
+            // (bounded, so that starts out of order cannot lead out of the workspace)
+            first = min(span.x, plan.shares - 1);
+            parts = min(span.y - first, plan.shares - 1 - first) + 1;
         } else if (r.kind != kv4::kPadding && turn == 0 && part == 0) {
             const float fill = r.kind == kv4::kBad ? __builtin_nanf("") : 0.0f;
             store4(dst, f32x4{fill, fill, fill, fill});
@@ -1521,9 +1522,12 @@ Cut cut_of(const ttl_kv4_cache *cache, const ttl_kv4_batch *batch, const ttl_kv4
     const uint64_t units = (chunks + p.unit - 1) / p.unit;
     // A workgroup takes a block whole where blocks are enough (1024 tokens at 2048: 61 against 87
     // us), or short enough for half as many (4 x 128 tokens at 1024: 35 against 47 us; but 512 at
-    // 8192: 198 against 137), or so many that finding a share would take long.
+    // 8192: 198 against 137), or so many that finding a share would take long, the units pass 31
+    // bits or the join a grid.
     const uint64_t all = uint64_t(p.blocks) * cache->kv_heads;
-    p.single = units == 1 || (cut.tile && (all >= slots || (2 * all >= slots && units <= 24))) || p.blocks > 1u << 16;
+    p.single = units == 1 || (cut.tile && (all >= slots || (2 * all >= slots && units <= 24))) ||
+               p.blocks > 1u << 16 || p.blocks * units > 1u << 31 ||
+               uint64_t(batch->tokens) * attention->heads > 1u << 26;
     if (p.single) {
         p.shares = p.blocks;
         return cut;
@@ -1557,8 +1561,7 @@ int run_attention(ttl_ctx *ctx, const ttl_kv4_cache *cache, const ttl_kv4_batch 
                 cut.workspace);
     TTL_REQUIRE(cut.workspace == 0 || (uintptr_t(workspace) & 255) == 0, TTL_ERR_INVALID,
                 "%s: the workspace must be 256-byte aligned", what);
-    const uint64_t groups = uint64_t(cut.plan.shares) * cache->kv_heads;
-    TTL_REQUIRE(groups * 2 * kThreads <= 0xffffffffu && uint64_t(batch->tokens) * attention->heads <= 0x7fffffffu, TTL_ERR_SHAPE,
+    TTL_REQUIRE(uint64_t(cut.plan.shares) * 2 * kThreads <= 0xffffffffu && uint64_t(batch->tokens) * attention->heads <= 0x7fffffffu, TTL_ERR_SHAPE,
                 "%s: %u tokens of %u heads are too many for one call", what, batch->tokens, attention->heads);
     TTL_HIP(hipSetDevice(ctx->device));
     const Cache c = kv4::view(cache);
