@@ -1069,17 +1069,39 @@ struct TileCodes {
     uint32_t w[HD / 32], scale;
 };
 
+// Where the tiles of one part (K or V) and index lie: what is the same in every chunk is added up
+// once, the tile's place in its chunk in the lane's offsets (pages of 64 and more hold it at a
+// fixed distance), so that a chunk costs few scalar instructions.
 template <int HD, int TP>
-__device__ __attribute__((always_inline)) inline void load_tile(const Cache &c, const Source<TP> &src, uint32_t chunk,
-                                                                uint32_t page, uint32_t index, bool v,
-                                                                const LaneOffsets<HD> &at, TileCodes<HD> &x) {
-    using L = Layout<HD>;
-    const uint32_t tile = TP == 1 ? chunk * kTiles + index : min(max(chunk * kTiles + index, src.lo / 16), src.hi / 16);
-    const uint32_t slot = (tile * 16) & ((1u << c.page_shift) - 1);
-    const uint8_t *rec = src.head + (page < c.pages ? page : 0u) * src.page_bytes;  // uniform
-    load_words<HD>(rec + (v ? L::v_codes(c.page_shift, slot) : L::k_codes(slot)) + at.code, x.w);
-    x.scale = (rec + (v ? L::v_scales(c.page_shift, slot) : L::k_scales(c.page_shift, slot)))[at.scale];
+struct TileSource {
+    const uint8_t *codes, *scales;  // uniform: of slot 0 of page 0
+    uint32_t code, scale;           // the lane's offsets
+    uint32_t page_bytes, mask;      // (kv_heads x record is below 2^24)
+    __device__ TileSource(const Cache &c, const Source<TP> &src, const LaneOffsets<HD> &at, uint32_t index, bool v)
+        : codes(src.head + (v ? Layout<HD>::v_codes(c.page_shift, 0) : 0)),
+          scales(src.head + (v ? Layout<HD>::v_scales(c.page_shift, 0) : Layout<HD>::k_scales(c.page_shift, 0))),
+          code(at.code + (TP == 1 ? index * 16 * Layout<HD>::code_bytes : 0)),
+          scale(at.scale + (TP == 1 ? index * 16 * Layout<HD>::scale_bytes : 0)),
+          page_bytes(c.kv_heads * c.record), mask((1u << c.page_shift) - 1) {}
+};
+
+template <int HD, int TP>
+__device__ __attribute__((always_inline)) inline void load_tile(const Cache &c, const Source<TP> &src,
+                                                                const TileSource<HD, TP> &from, uint32_t chunk,
+                                                                uint32_t page, uint32_t index, TileCodes<HD> &x) {
+    const uint32_t tile = TP == 1 ? chunk * kTiles : min(max(chunk * kTiles + index, src.lo / 16), src.hi / 16);
+    const uint32_t slot = (tile * 16) & from.mask;
+    const size_t at = size_t(page < c.pages ? page : 0u) * from.page_bytes;  // uniform
+    load_words<HD>(from.codes + (at + slot * Layout<HD>::code_bytes) + from.code, x.w);
+    x.scale = (from.scales + (at + slot * Layout<HD>::scale_bytes))[from.scale];
 }
+
+// Chunks from `first` on, `count` of them.
+struct ChunkRange {
+    uint32_t first, count;
+    __device__ ChunkRange(uint32_t from, uint32_t end) : first(from), count(end > from ? end - from : 0) {}
+    __device__ bool has(uint32_t chunk) const { return chunk - first < count; }
+};
 
 // The page of a tile of a chunk.
 template <int TP>
@@ -1132,7 +1154,12 @@ __device__ __attribute__((always_inline)) inline void do_tile(const Cache &c, co
     const int32_t p0 = k.position0 + int32_t((any ? own : 0u) / a.group);
     const int32_t p1 = k.position0 + int32_t((any ? own_last : 0u) / a.group);
     const int32_t window = a.window ? int32_t(a.window) : INT32_MAX;
-    const int32_t first_min = max(p0 + 1 - window, 0), first_max = max(p1 + 1 - window, 0);  // (p <= 2^30)
+    const uint32_t first_min = max(p0 + 1 - window, 0), first_max = max(p1 + 1 - window, 0);  // (p <= 2^30)
+    // the chunks of which some query sees a position, of which all see every one, and that lie
+    // in lo..hi whole
+    const ChunkRange needed(first_min / kChunk, any && p1 >= 0 ? uint32_t(p1) / kChunk + 1 : 0);
+    const ChunkRange whole((first_max + kChunk - 1) / kChunk, p0 >= 0 ? uint32_t(p0 + 1) / kChunk : 0);
+    const ChunkRange inside((k.lo + kChunk - 1) / kChunk, (k.hi + 1) / kChunk);
 #pragma unroll
     for (int qi = 0; qi < QT; ++qi) {
         const uint32_t query = own + 16 * qi + n, token = query / a.group;
@@ -1155,17 +1182,17 @@ __device__ __attribute__((always_inline)) inline void do_tile(const Cache &c, co
     }
 
     TileCodes<HD> x[KV];
+    const TileSource<HD, TP> from_k(c, src, at, index, is_v(0)), from_v(c, src, at, index, is_v(KV - 1));
     const auto load = [&](uint32_t chunk, uint32_t page) __attribute__((always_inline)) {
 #pragma unroll
         for (int part = 0; part < KV; ++part) {
-            load_tile<HD, TP>(c, src, chunk, page, index, is_v(part), at, x[part]);
+            load_tile<HD, TP>(c, src, part ? from_v : from_k, chunk, page, index, x[part]);
         }
     };
     // a page that is not there: keys read as NaN; values outside lo..hi are zeros
     const auto trim = [&](uint32_t chunk, uint32_t page) __attribute__((always_inline)) {
         const uint32_t p = chunk * kChunk + 16 * index + n;
-        const bool inside = chunk * kChunk >= src.lo && chunk * kChunk + kChunk - 1 <= src.hi;
-        if (!inside || page >= c.pages) {
+        if (!inside.has(chunk) || page >= c.pages) {
             const bool zero = p < src.lo || p > src.hi || page >= c.pages;
 #pragma unroll
             for (int part = 0; part < KV; ++part) {
@@ -1228,14 +1255,8 @@ __device__ __attribute__((always_inline)) inline void do_tile(const Cache &c, co
             }
         }
     };
-    const auto needed = [&](uint32_t chunk) __attribute__((always_inline)) {
-        const int32_t c0 = int32_t(chunk * kChunk);
-        return any && c0 <= p1 && c0 + int32_t(kChunk) > first_min;
-    };
     const auto soften = [&](uint32_t chunk, f32x4 (&s)[QT][kTiles]) __attribute__((always_inline)) {
-        const int32_t c0 = int32_t(chunk * kChunk);
-        const bool whole = c0 >= first_max && c0 + int32_t(kChunk) - 1 <= p0;
-        softmax_step<HD, M>(s, st, mine, whole, c0 + int32_t(4 * g), a.c);
+        softmax_step<HD, M>(s, st, mine, whole.has(chunk), int32_t(chunk * kChunk + 4 * g), a.c);
     };
     uint32_t chunk = first;
 #pragma unroll 1
@@ -1247,7 +1268,7 @@ __device__ __attribute__((always_inline)) inline void do_tile(const Cache &c, co
             break;
         }
         f32x4 s[QT][kTiles];
-        if (needed(chunk)) {
+        if (needed.has(chunk)) {
             scores(buf, s);
         }
         // the next chunk into the other buffer, whose readers are behind the last barrier (at the
@@ -1256,7 +1277,7 @@ __device__ __attribute__((always_inline)) inline void do_tile(const Cache &c, co
         page = next;
         next = tile_page<TP>(c, src, min(chunk + 3, end - 1), index);
         load(min(chunk + 2, end - 1), page);
-        if (needed(chunk)) {
+        if (needed.has(chunk)) {
             soften(chunk, s);
             weigh_values<HD, f16x8, PP, M>(sh.v[buf], s, st, n, g);
         }
@@ -1289,7 +1310,7 @@ __device__ __attribute__((always_inline)) inline void do_tile(const Cache &c, co
             }
         }
         __syncthreads();
-        if (needed(chunk)) {
+        if (needed.has(chunk)) {
             f32x4 s[QT][kTiles];
             scores(0, s);
             soften(chunk, s);
