@@ -589,7 +589,7 @@ typedef struct {
  * than max_length, or needs a page outside the pool, gets NaN. */
 typedef struct {
     uint32_t sequences;         /* 0..2^20                                              */
-    uint32_t tokens;            /* rows, 0..2^24                                        */
+    uint32_t tokens;            /* rows, 0..2^24, and what fits a launch (2^32 threads; refused) */
     uint32_t table_stride;      /* page-table entries per sequence                      */
     uint32_t max_length;        /* at least every length; at most table_stride x page_positions and 2^30 */
     const int32_t *page_table;  /* int32 [sequences][table_stride]                      */

@@ -159,3 +159,11 @@ def test_reference_blocks():
     a, err = np.abs(r) / unit, np.abs(R.values(code, byte) - r) / unit
     assert a.max() < 7.0 and a.max(1).min() >= 3.5
     assert (err <= np.where(a < 2, 0.25, np.where(a < 4, 0.5, 1.0))).all()
+
+
+def test_calls_past_a_launch_are_refused():
+    """2^24 rows: more threads than one launch counts."""
+    c, b = cache(), batch(sequences=1, tokens=1 << 24, starts=P)
+    assert store(c, b) == SHAPE and b"too many" in LIB.ttl_last_error()
+    assert LIB.ttl_kv4_dequantize(CTX, C.byref(c), C.byref(b), P, P) == SHAPE
+    assert attend(c, b, attention(heads=64 * 8), prefill=True) == SHAPE
