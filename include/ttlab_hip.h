@@ -620,7 +620,7 @@ size_t ttl_kv4_pool_bytes(const ttl_kv4_cache *cache);
  * Bias and rotation are computed in 64 bits, so q is rounded once and a code is the nearest
  * one of the exact value.  A row at a position from rope_positions on counts as one of a too
  * long sequence: nothing is stored for such rows.  No two rows may share a position of a
- * page.  qkv, bias, rope and q 16-byte aligned. */
+ * page.  qkv, bias, rope and q 16-byte aligned, q apart from the others. */
 #define TTL_QKV_PLAIN 0
 #define TTL_QKV_TILED 1
 int ttl_qkv_rope_store_kv4(ttl_ctx *ctx, const ttl_kv4_cache *cache, const ttl_kv4_batch *batch, uint32_t heads,
@@ -638,7 +638,7 @@ size_t ttl_attention_kv4_workspace_bytes(const ttl_kv4_cache *cache, const ttl_k
                                          const ttl_kv4_attention *attention);
 /* out = softmax(scale q k, sink) v of one token per sequence (batch->starts NULL) at its last
  * position, the sink in the maximum and the denominator only (model.cpp:270-281): q_dev and
- * out_dev [sequences][heads][head_dim] of attention->dtype, 16-byte aligned.  A query with a
+ * out_dev [sequences][heads][head_dim] of attention->dtype, 16-byte aligned and apart.  A query with a
  * value that is not finite gives NaN, as does one that sees a NaN block; masked positions
  * have no influence whatever they hold.  Scores are f32 sums of exact products (f32 queries
  * as three bf16 planes, 24 bits), their maxima, the exponentials' sums and the outputs f32.  The
