@@ -59,7 +59,8 @@ constexpr uint32_t kF16First = 104, kF16Last = 140;                  // scale by
 constexpr float kWeightShift = 7.0f;                                // weights are held times 2^7
 
 // How a wave's 16 columns are used (M): kHalf for 8 queries or fewer, columns 8..15 the same
-// queries on the other half of the chunk (so that no lane weighs scores that nobody asked for);
+// queries on the other half of the chunk (so that no lane weighs scores that nobody asked for:
+// 128 f32 sequences at 4096 in 72.9 instead of 74.7 us, level in bf16);
 // kOne and kTwo for 16 queries, and 32 in two column tiles.
 constexpr int kHalf = 0, kOne = 1, kTwo = 2;
 template <int M>
@@ -1502,7 +1503,12 @@ uint32_t resident_groups(uint32_t head_dim, int dtype) {
 }
 
 // The cut of a checked call, by the queries that a sequence has on average: few share a
-// workgroup's waves, from kTileFrom on each wave has its own.
+// workgroup's waves, from kTileFrom on each wave has its own.  Heads of 64 over long contexts
+// fill a wave with less: from kTileFromLong on where a query sees more than kLongChunks (64
+// sequences of 128 queries, bf16: at 2048 the split kernel takes 97 against 116 us, with a window
+// of 128 43 against 33; of 192 queries at 1024 98 against 79, 8 of 256 at 4096 47 against 48, 64
+// of 256 with the window 76 against 43; heads of 128, 8 sequences of 200 queries at 4096: 52
+// against 43).
 struct Cut {
     bool tile;
     int mode;
@@ -1510,7 +1516,8 @@ struct Cut {
     uint32_t most_parts;  // of a block
     size_t workspace;
 };
-constexpr uint64_t kTileFrom = 64;
+constexpr uint64_t kTileFrom = 64, kTileFromLong = 256;
+constexpr uint32_t kLongChunks = 24;
 constexpr uint64_t kCus = 256;
 Cut cut_of(const ttl_kv4_cache *cache, const ttl_kv4_batch *batch, const ttl_kv4_attention *attention) {
     const uint32_t group = attention->heads / cache->kv_heads;
@@ -1519,7 +1526,11 @@ Cut cut_of(const ttl_kv4_cache *cache, const ttl_kv4_batch *batch, const ttl_kv4
     const uint64_t queries = uint64_t(batch->tokens) * group;  // of a key/value head
     const uint64_t mean = queries / batch->sequences;
     Plan &p = cut.plan;
-    cut.tile = batch->starts && mean >= kTileFrom;
+    const uint64_t seen = attention->window
+                              ? std::min<uint64_t>(batch->max_length, uint64_t(attention->window) + mean / group)
+                              : batch->max_length;
+    const bool fits = cache->head_dim == 64 && seen / kChunk > kLongChunks;
+    cut.tile = batch->starts && mean >= (fits ? kTileFromLong : kTileFrom);
     uint64_t slots = 0;
     if (cut.tile) {
         const auto take = [&](auto tile) {
@@ -1554,7 +1565,7 @@ Cut cut_of(const ttl_kv4_cache *cache, const ttl_kv4_batch *batch, const ttl_kv4
     // 8192: 198 against 137), or so many that finding a share would take long, the units pass 31
     // bits or the join a grid.
     const uint64_t all = uint64_t(p.blocks) * cache->kv_heads;
-    p.single = units == 1 || (cut.tile && (all >= slots || (2 * all >= slots && units <= 24))) ||
+    p.single = units == 1 || (cut.tile && (all >= slots || (2 * all >= slots && units <= kLongChunks))) ||
                p.blocks > 1u << 16 || p.blocks * units > 1u << 31 ||
                uint64_t(batch->tokens) * attention->heads > 1u << 26;
     if (p.single) {
