@@ -1517,7 +1517,7 @@ struct Cut {
     size_t workspace;
 };
 constexpr uint64_t kTileFrom = 64, kTileFromLong = 256;
-constexpr uint32_t kLongChunks = 24;
+constexpr uint32_t kLongChunks = 24, kShortChunks = 8;
 constexpr uint64_t kCus = 256;
 Cut cut_of(const ttl_kv4_cache *cache, const ttl_kv4_batch *batch, const ttl_kv4_attention *attention) {
     const uint32_t group = attention->heads / cache->kv_heads;
@@ -1562,10 +1562,11 @@ Cut cut_of(const ttl_kv4_cache *cache, const ttl_kv4_batch *batch, const ttl_kv4
     const uint64_t units = (chunks + p.unit - 1) / p.unit;
     // A workgroup takes a block whole where blocks are enough (1024 tokens at 2048: 61 against 87
     // us), or short enough for half as many (4 x 128 tokens at 1024: 35 against 47 us; but 512 at
-    // 8192: 198 against 137), or so many that finding a share would take long, the units pass 31
+    // 8192: 198 against 137), or so short that the join costs more than a workgroup's walk (a
+    // prompt of 300: 13 against 26 us; two of 100 at 1400, f32: 46 against 38), or so many that finding a share would take long, the units pass 31
     // bits or the join a grid.
     const uint64_t all = uint64_t(p.blocks) * cache->kv_heads;
-    p.single = units == 1 || (cut.tile && (all >= slots || (2 * all >= slots && units <= kLongChunks))) ||
+    p.single = units == 1 || (cut.tile && (all >= slots || (2 * all >= slots && units <= kLongChunks) || units <= kShortChunks)) ||
                p.blocks > 1u << 16 || p.blocks * units > 1u << 31 ||
                uint64_t(batch->tokens) * attention->heads > 1u << 26;
     if (p.single) {
