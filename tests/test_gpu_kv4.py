@@ -847,3 +847,47 @@ def test_captured_prompts(dev, held, news):
         a, b = (o.download(np.uint16, tokens * heads * 64) for o in outs)
         assert np.array_equal(a, b) and (a != 0x5a5a).any(), step
     graph.free()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("prefill", [False, True])
+@pytest.mark.parametrize("window", [0, 200])
+def test_widest_group(dev, held, dtype, prefill, window):
+    """64 query heads a key/value head, the most there are."""
+    rng = np.random.default_rng(51)
+    heads, lengths, news = 128, [900, 1, 0, 2100], [3, 1, 1, 2]
+    pool = R.Pool(60, 2, 64, 64).randomise(rng)
+    table = R.tables(rng, lengths, 64, 60)
+    each = news if prefill else [1] * 4
+    q, qb = to_dtype(rng.standard_normal((sum(each), heads, 64)), dtype)
+    sinks = rng.standard_normal(heads).astype(np.float32)
+    got = run_attention(dev, held, held.up(pool.bytes), pool, table, lengths, news if prefill else None, qb, heads,
+                        dtype, window, 0.125, sinks)
+    check_attention(got, q, pool, table, lengths, each, heads, dtype, window, 0.125, sinks)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,page", [(64, 8, 64, 64), (64, 8, 64, 32), (20, 4, 128, 64), (20, 4, 128, 16)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("new,length", [(200, 300), (120, 2500)])
+@pytest.mark.parametrize("missing", [-1, 1 << 30])
+def test_a_missing_page_in_a_prompt(dev, held, heads, kv_heads, hd, page, dtype, new, length, missing):
+    """NaN for the rows that see it, through a window; the others as without it."""
+    rng = np.random.default_rng(53)
+    window = 40
+    lengths, news = [length, 64], [new, 64]
+    pages = sum(-(-n // page) for n in lengths)
+    pool = R.Pool(pages, kv_heads, hd, page).randomise(rng)
+    table = R.tables(rng, lengths, page, pages)
+    gone = (length - 150) // page                       # the page of a position inside the prompt
+    q, qb = to_dtype(rng.standard_normal((new + 64, heads, hd)), dtype)
+    broken = table.copy()
+    broken[0, gone] = missing
+    pb = held.up(pool.bytes)
+    whole, got = (run_attention(dev, held, pb, pool, t, lengths, news, qb, heads, dtype, window, 0.125, None)
+                  for t in (table, broken))
+    at = np.arange(length - new, length)
+    sees = (at >= gone * page) & (at - window + 1 < (gone + 1) * page)
+    assert sees.any() and not sees.all()
+    assert np.isnan(got[:new][sees]).all()
+    assert np.array_equal(got[:new][~sees], whole[:new][~sees]) and np.array_equal(got[new:], whole[new:])
+    check_attention(whole, q, pool, table, lengths, news, heads, dtype, window, 0.125, None)
