@@ -26,8 +26,8 @@
 // Maxima, sums and outputs are f32.
 //
 // What bounds them (a large copy moves 5.1 TB/s here, a large f16 product 1.18 PFLOP/s).  One
-// token a sequence: the codes are read once; 128 sequences at 4096 (289 MB, f32 queries) take 73
-// us with their join, 4.0 TB/s, 64 ragged ones up to 8192 (151 MB, bf16) 49 us, 3.1 TB/s: the vector
+// token a sequence: the codes are read once; 128 sequences at 4096 (289 MB, f32 queries) take 73..76
+// us with their join, 3.8 to 4.0 TB/s, 64 ragged ones up to 8192 (151 MB, bf16) 49 us, 3.1 TB/s: the vector
 // instructions of conversion and softmax, a third of the cycles, against loads that 2 or 3
 // waves a SIMD keep in flight.  Prompts: the vector instructions, half of the cycles (an exponential a
 // score costs as much as three multiply-adds, a conversion as one and a half), next to the
@@ -234,7 +234,8 @@ __device__ __attribute__((always_inline)) inline void load_codes(const Cache &c,
             codes = rec + (V ? L::v_codes(c.page_shift, slot) : L::k_codes(slot));
             scales = rec + (V ? L::v_scales(c.page_shift, slot) : L::k_scales(c.page_shift, slot));
         }
-        const uint32_t tile_code = TP == 1 ? i * 16 * L::code_bytes : 0, tile_scale = TP == 1 ? i * 16 * L::scale_bytes : 0;
+        const uint32_t tile_code = TP == 1 ? i * 16 * L::code_bytes : 0;
+        const uint32_t tile_scale = TP == 1 ? i * 16 * L::scale_bytes : 0;
         load_words<HD>(codes + (at.code + tile_code), x.w[i]);
         x.scale[i] = scales[at.scale + tile_scale];
     }
@@ -1044,8 +1045,8 @@ attention_split_kernel(Cache c, Batch b, Params a, Plan plan, const T *__restric
 
 // ---- many queries: the waves of a workgroup share the chunks, each with queries of its own --------
 //
-// Each wave converts a tile of 16 positions of the chunk, K to bf16 and V to f16 in LDS, where
-// all four read it; two buffers, so that the next chunk is converted while this one is used,
+// The waves convert the chunk's tiles of 16 positions, K to bf16 and V to f16 in LDS, where all
+// of them read them; two buffers, so that the next chunk is converted while this one is used,
 // with one barrier a chunk.  A chunk with values outside the f16 path's range is found when it
 // is converted (a flag a wave, beside the buffer), and the rest of the walk takes the bf16 path.
 
@@ -1372,7 +1373,8 @@ __device__ __attribute__((always_inline)) inline void do_tile(const Cache &c, co
 }
 
 template <int HD, class T, int TP>
-__global__ __launch_bounds__((Tile<HD, T>::threads)) __attribute__((amdgpu_waves_per_eu(Tile<HD, T>::waves_per_simd))) void
+__global__ __launch_bounds__((Tile<HD, T>::threads))
+    __attribute__((amdgpu_waves_per_eu(Tile<HD, T>::waves_per_simd))) void
 attention_tile_kernel(Cache c, Batch b, Params a, Plan plan, const T *__restrict__ q, T *__restrict__ out) {
     __shared__ __attribute__((aligned(16))) TileShared<HD, T> sh;
     do_share<HD, T, Tile<HD, T>::waves>(
@@ -1563,11 +1565,11 @@ Cut cut_of(const ttl_kv4_cache *cache, const ttl_kv4_batch *batch, const ttl_kv4
     // A workgroup takes a block whole where blocks are enough (1024 tokens at 2048: 61 against 87
     // us), or short enough for half as many (4 x 128 tokens at 1024: 35 against 47 us; but 512 at
     // 8192: 198 against 137), or so short that the join costs more than a workgroup's walk (a
-    // prompt of 300: 13 against 26 us; two of 100 at 1400, f32: 46 against 38), or so many that finding a share would take long, the units pass 31
-    // bits or the join a grid.
+    // prompt of 300: 13 against 26 us; two of 100 at 1400, f32: 46 against 38), or so many that
+    // finding a share would take long, the units pass 31 bits or the join a grid.
     const uint64_t all = uint64_t(p.blocks) * cache->kv_heads;
-    p.single = units == 1 || (cut.tile && (all >= slots || (2 * all >= slots && units <= kLongChunks) || units <= kShortChunks)) ||
-               p.blocks > 1u << 16 || p.blocks * units > 1u << 31 ||
+    const bool whole = all >= slots || (2 * all >= slots && units <= kLongChunks) || units <= kShortChunks;
+    p.single = units == 1 || (cut.tile && whole) || p.blocks > 1u << 16 || p.blocks * units > 1u << 31 ||
                uint64_t(batch->tokens) * attention->heads > 1u << 26;
     if (p.single) {
         p.shares = p.blocks;
@@ -1602,7 +1604,9 @@ int run_attention(ttl_ctx *ctx, const ttl_kv4_cache *cache, const ttl_kv4_batch 
                 cut.workspace);
     TTL_REQUIRE(cut.workspace == 0 || (uintptr_t(workspace) & 255) == 0, TTL_ERR_INVALID,
                 "%s: the workspace must be 256-byte aligned", what);
-    TTL_REQUIRE(uint64_t(cut.plan.shares) * 2 * kThreads <= 0xffffffffu && uint64_t(batch->tokens) * attention->heads <= 0x7fffffffu, TTL_ERR_SHAPE,
+    TTL_REQUIRE(uint64_t(cut.plan.shares) * 2 * kThreads <= 0xffffffffu &&  // (a launch's threads)
+                    uint64_t(batch->tokens) * attention->heads <= 0x7fffffffu,
+                TTL_ERR_SHAPE,
                 "%s: %u tokens of %u heads are too many for one call", what, batch->tokens, attention->heads);
     TTL_HIP(hipSetDevice(ctx->device));
     const Cache c = kv4::view(cache);
