@@ -891,3 +891,27 @@ def test_a_missing_page_in_a_prompt(dev, held, heads, kv_heads, hd, page, dtype,
     assert np.isnan(got[:new][sees]).all()
     assert np.array_equal(got[:new][~sees], whole[:new][~sees]) and np.array_equal(got[new:], whole[new:])
     check_attention(whole, q, pool, table, lengths, news, heads, dtype, window, 0.125, None)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,page", [(64, 8, 64, 64), (8, 2, 64, 16), (5, 5, 128, 32), (20, 4, 128, 64),
+                                                    (3, 3, 64, 128)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("with_sinks", [False, True])
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("capacity", [256, 1500])       # blocks taken whole, and divided
+def test_prompts_with_more_rows_than_positions(dev, held, heads, kv_heads, hd, page, dtype, with_sinks, window,
+                                               capacity):
+    """Rows before position 0 next to rows that see positions, in prompts long enough for a wave to
+    have queries of its own: zeros for the ones, the others as they are without them."""
+    rng = np.random.default_rng(61 + heads + window)
+    news = [130, 131, 97, 170]
+    lengths = [n - more for n, more in zip(news, (3, 7, 20, 30))]
+    pages = sum(-(-n // page) for n in lengths)
+    pool = R.Pool(pages, kv_heads, hd, page).randomise(rng)
+    table = R.tables(rng, lengths, page, pages, capacity // page + 1)
+    q, qb = to_dtype(rng.standard_normal((sum(news), heads, hd)) * 1.5, dtype)
+    sinks = rng.standard_normal(heads).astype(np.float32) if with_sinks else None
+    scale = float(np.float32(hd ** -0.5))
+    got = run_attention(dev, held, held.up(pool.bytes), pool, table, lengths, news, qb, heads, dtype, window, scale,
+                        sinks, max_length=capacity)
+    check_attention(got, q, pool, table, lengths, news, heads, dtype, window, scale, sinks)

@@ -1163,8 +1163,11 @@ __device__ __attribute__((always_inline)) inline void do_tile(const Cache &c, co
     const bool any = own < limit;
     const int32_t p0 = k.position0 + int32_t((any ? own : 0u) / a.group);
     const int32_t p1 = k.position0 + int32_t((any ? own_last : 0u) / a.group);
-    const int32_t window = a.window ? int32_t(a.window) : INT32_MAX;
-    const uint32_t first_min = max(p0 + 1 - window, 0), first_max = max(p1 + 1 - window, 0);  // (p <= 2^30)
+    // the first position that one at p sees (p may be negative: rows before position 0)
+    const auto first_seen = [&](int32_t p) __attribute__((always_inline)) {
+        return a.window && p + 1 > int32_t(a.window) ? p + 1 - int32_t(a.window) : 0;
+    };
+    const uint32_t first_min = uint32_t(first_seen(p0)), first_max = uint32_t(first_seen(p1));
     // the chunks of which some query sees a position, of which all see every one, and that lie
     // in lo..hi whole
     const ChunkRange needed(first_min / kChunk, any && p1 >= 0 ? uint32_t(p1) / kChunk + 1 : 0);
@@ -1176,7 +1179,7 @@ __device__ __attribute__((always_inline)) inline void do_tile(const Cache &c, co
         const bool there = query < limit;
         const int32_t position = k.position0 + int32_t(token);
         mine[qi].last = there ? position : -1;
-        mine[qi].first = max(position + 1 - window, 0);
+        mine[qi].first = first_seen(position);
         const uint32_t row = k.row0 + (there ? token : 0u);
         const uint32_t head = kv_head * a.group + (there ? query - token * a.group : 0u);
         RawQuery<HD, T> raw;
