@@ -319,7 +319,7 @@ def _run_own(st):
                                          sinks=None if t["sinks"] is None else t["sinks"].data_ptr())
             need = dev.attention_kv4_workspace_bytes(cache, batch, st.heads)
             st.ws = torch.empty(max(need, 16), dtype=torch.uint8, device="cuda")
-            torch.cuda.synchronize()  # the library works on a stream of its own
+        torch.cuda.synchronize()  # the library works on a stream of its own: the inputs have to be there
     dtype, cache, batch = st.plan
     if c["kind"] == "store":
         dev.qkv_rope_store_kv4(cache, batch, c["heads"], _ptr(t["qkv"]), lib.TTL_DTYPE_F32, _ptr(t["bias"]),
