@@ -642,9 +642,9 @@ size_t ttl_attention_kv4_workspace_bytes(const ttl_kv4_cache *cache, const ttl_k
  * value that is not finite gives NaN, as does one that sees a NaN block; masked positions
  * have no influence whatever they hold.  Scores are f32 sums of exact products (f32 queries
  * as three bf16 planes, 24 bits), their maxima, the exponentials' sums and the outputs f32.  The
- * weights go into the product with V as f16 for a bf16 output (2^-11 of a weight) and as two
- * f16 planes for an f32 one (2^-22; weights far below the largest seen so far lose at most 2^-32
- * of that one).  Results depend on nothing but the call: the same one gives the same bits.
+ * weights go into the product with V as bf16 planes, three for an f32 output (2^-24 of a weight),
+ * two for a bf16 one (2^-16); weights below 2^-118 of the largest seen so far may count as zero.
+ * Results depend on nothing but the call: the same one gives the same bits.
  * workspace_dev is caller-owned, 256-byte aligned, of the size above; calls sharing one must
  * not overlap. */
 int ttl_attention_decode_kv4(ttl_ctx *ctx, const ttl_kv4_cache *cache, const ttl_kv4_batch *batch,

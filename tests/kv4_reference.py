@@ -176,3 +176,14 @@ def allowance(ref, mag, smax, vsum, n, hd, bf16):
     if bf16:
         return mag * (rel + 2.0 ** -11) * 1.01 + 2.0 ** -8 * np.abs(ref) * 1.01 + floor
     return mag * (rel + 2.0 ** -22) * 1.01 + floor
+
+
+def close_allowance(ref, mag, smax, vsum, n, hd, bf16):
+    """allowance() for weights that keep f32's range: bf16 planes, each the nearest bf16 of what the
+    ones before leave.  A plane leaves at most half a step, 2^-8 of what it takes, so three leave
+    2^-24 of a weight (an f32 output) and two 2^-16 (a bf16 one).  Scores, sums and an output's
+    own rounding as there.  The largest weight so far is held as 2^-8 at least, and what is held
+    below f32's smallest normal value, 2^-126, may be lost: 2^-118 |v| for each position seen."""
+    u = 2.0 ** -24
+    rel = 2.0 * (hd + 8) * u * smax[..., None] + (2 * n + 32) * u + (2.0 ** -16 if bf16 else 2.0 ** -24)
+    return mag * rel * 1.01 + (2.0 ** -8 * np.abs(ref) * 1.01 if bf16 else 0.0) + 2.0 ** -118 * vsum + 2.0 ** -133

@@ -915,3 +915,65 @@ def test_prompts_with_more_rows_than_positions(dev, held, heads, kv_heads, hd, p
     got = run_attention(dev, held, held.up(pool.bytes), pool, table, lengths, news, qb, heads, dtype, window, scale,
                         sinks, max_length=capacity)
     check_attention(got, q, pool, table, lengths, news, heads, dtype, window, scale, sinks)
+
+
+# ---- the weights' bits -------------------------------------------------------------------------------
+#
+# (heads, kv heads, head width, new tokens; None: decode) that take each of the kernels' ways of working
+WAYS = [(8, 1, 64, None), (8, 1, 64, [2]), (8, 1, 64, [4]), (8, 1, 64, [70]), (8, 1, 64, [300]), (8, 1, 128, None),
+        (8, 1, 128, [2]), (8, 1, 128, [4]), (8, 1, 128, [70])]
+
+
+def check_close(got, q, pool, table, lengths, news, heads, dtype, window, scale, sinks):
+    row = 0
+    for s, (n, m) in enumerate(zip(lengths, news)):
+        first = max(0, n - m + 1 - window) if window else 0
+        k, v = pool.get(table[s], np.arange(first, n))
+        ref, mag, smax, vsum = R.attention(q[row:row + m], k, v, np.arange(n - m, n), first, window, scale, sinks)
+        tol = R.close_allowance(ref, mag, smax, vsum, n - first, pool.hd, dtype == BF16)
+        off = np.abs(got[row:row + m] - ref)
+        assert (off <= tol).all(), (s, n, m, float((off / np.maximum(tol, 1e-300)).max()))
+        row += m
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,news", WAYS)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("top", [0, 1900, 3600])
+def test_small_weights_count(dev, held, heads, kv_heads, hd, news, dtype, top):
+    """One key up to 60 nats above thousands of equal ones, with a v of zero in half the dims: what
+    is left there is the small weights' sum."""
+    n, page = 4001, 64
+    pool = R.Pool(63, kv_heads, hd, page)
+    table = np.arange(63, dtype=np.int32)[None]
+    for codes, scales, x in ((pool.kc, pool.ks, 0.0), (pool.vc, pool.vs, 1.0)):
+        code, byte = R.quantise(np.full(hd, x))
+        codes[...], scales[...] = R.pack(code), byte
+    k, v = np.zeros((kv_heads, hd)), np.ones((kv_heads, hd))
+    k[:, 0], v[:, :hd // 2] = 1.0, 0.0
+    pool.put(table[0], top, k, v)
+    rows = news[0] if news else 1
+    x = np.zeros((rows, heads, hd))
+    x[:, :, 0] = 8.0 * np.array([0, 10, 18, 21, 23, 30, 45, 60])   # (bf16 holds these)
+    q, qb = to_dtype(x, dtype)
+    got = run_attention(dev, held, held.up(pool.bytes), pool, table, [n], news, qb, heads, dtype, 0, 0.125, None)
+    check_close(got, q, pool, table, [n], news or [1], heads, dtype, 0, 0.125, None)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,news", WAYS)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_weights_keep_their_bits(dev, held, heads, kv_heads, hd, news, dtype):
+    """Values of alternating sign under nearly equal weights: what is left of a sum is the weights'
+    differences, far below their own rounding to 11 bits."""
+    rows, page = news[0] if news else 1, 64
+    n = max(rows, 2)
+    pool = R.Pool(5, kv_heads, hd, page)
+    table = np.arange(5, dtype=np.int32)[None]
+    for p in range(n):
+        k = np.zeros((kv_heads, hd))
+        k[:, 0] = (p + 1) % 2
+        pool.put(table[0], p, k, np.full((kv_heads, hd), 1.0 - 2.0 * (p % 2)))
+    x = np.zeros((rows, heads, hd))
+    x[:, :, 0] = 8.0 * np.linspace(0.001, 0.011, rows * heads).reshape(rows, heads)
+    q, qb = to_dtype(x, dtype)
+    got = run_attention(dev, held, held.up(pool.bytes), pool, table, [n], news, qb, heads, dtype, 0, 0.125, None)
+    check_close(got, q, pool, table, [n], news or [1], heads, dtype, 0, 0.125, None)

@@ -4,7 +4,7 @@
 // (token, head) and taken in blocks.  Per chunk of 64 positions and tile of 16 queries:
 //  - S^T (positions x queries) = K Q^T on v_mfma_f32_16x16x32_bf16, then the online softmax of
 //    each query (a column of S^T) in units of log 2;
-//  - O^T (dims x queries) += V^T P^T on v_mfma_f32_16x16x32_f16.
+//  - O^T (dims x queries) += V^T P^T on the same instruction.
 // Lane (n, g) = (l % 16, l / 16) of a wave holds 8 values of A row n and B column n for 8 of the
 // instruction's 32 K indices, the same for both, and receives D rows 4g..4g+3 of column n.
 //
@@ -12,18 +12,16 @@
 // lie next to each other in the cache and in one block, so the codes go from memory to bf16 in
 // the lane that multiplies them, the scale folded in (exact: E2M1 x 2^e is a bf16).
 // V: its K index is the position, and neighbouring codes of a lane's operand would have
-// different scales, so V is converted in the layout it is stored in (dims side by side) to f16
+// different scales, so V is converted in the layout it is stored in (dims side by side) to bf16
 // in LDS, and read back transposed (ds_read_b64_tr_b16: 16 lanes take a 4 x 16 block, lane n its
 // column n).  The lane's 8 positions are those of its own rows of two S^T tiles, so the
 // weights never leave their registers.
 //
-// Numerics: K and bf16 queries are exact in bf16, f32 queries three bf16 planes (24 bits).  The
-// weights, relative to a large one held as 2^7, are rounded to f16 for a bf16 output (2^-11, an
-// eighth of the output's own rounding) and to two f16 planes for an f32 one (2^-22; weights
-// below 2^-21 of the large one lose more of themselves, 2^-32 of it).  V is exact in f16 where
-// its scale bytes are 104..140 (subnormals included: the matrix cores keep them); a chunk with
-// another one takes V as bf16, exact for every byte, and three bf16 planes of the weights.
-// Maxima, sums and outputs are f32.
+// Numerics: K, V and bf16 queries are exact in bf16, f32 queries three bf16 planes (24 bits).  The
+// weights go into the product with V as bf16 planes, which keep f32's range: three for an f32
+// output (2^-24 of a weight), two for a bf16 one (2^-16, where the output's own rounding is 2^-8).
+// Maxima, sums and outputs are f32.  A NaN block of V would reach rows that do not see it (a weight
+// of zero times NaN), so its values are zeros in LDS and the queries that see it are noted apart.
 //
 // What bounds them (a large copy moves 5.1 TB/s here, a large f16 product 1.18 PFLOP/s).  One
 // token a sequence: the codes are read once; 128 sequences at 4096 (289 MB, f32 queries) take 73..76
@@ -31,7 +29,8 @@
 // instructions of conversion and softmax, a third of the cycles, against loads that 2 or 3
 // waves a SIMD keep in flight.  Prompts: the vector instructions, half of the cycles (an exponential a
 // score costs as much as three multiply-adds, a conversion as one and a half), next to the
-// products' fifth: 4096 tokens of 64 bf16 heads of 64 take 251 us, 548 TFLOP/s.
+// products' quarter: 4096 tokens of 64 bf16 heads of 64 take 312 us, 440 TFLOP/s (251 with the weights
+// as one f16 plane, which lost those 2^-32 and less of the largest).
 #include "ttl_kv4.hpp"
 #include "ttl_mfma.hpp"
 
@@ -45,7 +44,6 @@ using kv4::Batch;
 using kv4::Cache;
 using kv4::Layout;
 using mf::bf16x8;
-using mf::f16x8;
 using mf::f32x4;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
@@ -55,7 +53,6 @@ typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 constexpr uint32_t kChunk = 64, kTiles = kChunk / 16;
 constexpr uint32_t kWaves = 4, kThreads = kWaves * 64;
 constexpr float kLog2e = 0x1.715476p+0f, kLog2eLo = 0x1.4ae0cp-26f;  // log2 e = their sum
-constexpr uint32_t kF16First = 104, kF16Last = 140;                  // scale bytes of V on the f16 path
 constexpr float kWeightShift = 7.0f;                                // weights are held times 2^7
 
 // How a wave's 16 columns are used (M): kHalf for 8 queries or fewer, columns 8..15 the same
@@ -307,8 +304,8 @@ struct Query {
 };
 
 // Scores to weights, in place.  The offset follows the largest score lazily: it is set anew (and
-// what is there rescaled) only when a weight would pass 2^15, before which none leaves the f16
-// range, or before any score was seen (its weights would then be infinite).
+// what is there rescaled) only when a weight would pass 2^15, or before any score was seen (its
+// weights would then be infinite).
 // `at`: the position of the lane's first score.
 template <int HD, int M>
 __device__ __attribute__((always_inline)) inline void softmax_step(f32x4 (&s)[Mode<M>::columns][Mode<M>::tiles],
@@ -377,27 +374,15 @@ __device__ __attribute__((always_inline)) inline void softmax_step(f32x4 (&s)[Mo
     }
 }
 
-template <class V>
-struct Planes;
-template <>
-struct Planes<f16x8> {
-    typedef _Float16 type2 __attribute__((ext_vector_type(2)));
-};
-template <>
-struct Planes<bf16x8> {
-    typedef __bf16 type2 __attribute__((ext_vector_type(2)));
-};
-
-// 8 f32 values as P planes, each the remainder rounded.
-template <class V, int P>
-__device__ __attribute__((always_inline)) inline void split(const float (&x)[8], V (&out)[P]) {
-    using T2 = typename Planes<V>::type2;
+// 8 f32 values as P bf16 planes, each the remainder rounded.
+template <int P>
+__device__ __attribute__((always_inline)) inline void split(const float (&x)[8], bf16x8 (&out)[P]) {
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
         float a = x[e], b = x[e + 1];
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            const T2 w = __builtin_convertvector(f32x2{a, b}, T2);
+            const mf::bf16x2 w = __builtin_convertvector(f32x2{a, b}, mf::bf16x2);
             out[p][e] = w[0];
             out[p][e + 1] = w[1];
             if (p + 1 < P) {
@@ -419,7 +404,7 @@ __device__ __attribute__((always_inline)) inline uint32_t piece_at(uint32_t row,
     return row * HD + (((c / 2) ^ turn) * 2 + ((c % 2) ^ (row / 8 % 2))) * 8;
 }
 
-template <int HD, class V>
+template <int HD>
 __device__ __attribute__((always_inline)) inline void stage_values(uint16_t *lds, const Codes<HD> &v, uint32_t n,
                                                                    uint32_t g) {
 #pragma unroll
@@ -428,77 +413,37 @@ __device__ __attribute__((always_inline)) inline void stage_values(uint16_t *lds
 #pragma unroll
         for (int s = 0; s < HD / 32; ++s) {
             // (rows 16 apart are turned alike)
-            *reinterpret_cast<V *>(lds + piece_at<HD>(n, g * (HD / 32) + s) + 16 * i * HD) =
-                mf::decode_as<V>(v.w[i][s], scale);
+            *reinterpret_cast<bf16x8 *>(lds + piece_at<HD>(n, g * (HD / 32) + s) + 16 * i * HD) =
+                mf::decode_step(v.w[i][s], scale);
         }
     }
 }
 
 // A operand of K step h (positions of tiles 2h and 2h + 1) and dims 16 mt..: the lane's own
 // rows 4g..4g+3 of both tiles, of dim 16 mt + n.
-template <int HD, class V>
-__device__ __attribute__((always_inline)) inline V value_fragment(const uint16_t *lds, int h, int mt, uint32_t n,
-                                                                  uint32_t g) {
+template <int HD>
+__device__ __attribute__((always_inline)) inline bf16x8 value_fragment(const uint16_t *lds, int h, int mt, uint32_t n,
+                                                                       uint32_t g) {
     typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
     const uint16_t *p = lds + piece_at<HD>(4 * g + n / 4, 2 * mt + n % 4 / 2) + 4 * (n % 2) + 32 * h * HD;
     const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p));
     const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4 *)(p + 16 * HD));
     typedef short s16x8 __attribute__((ext_vector_type(8)));
-    return __builtin_bit_cast(V, s16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
+    return __builtin_bit_cast(bf16x8, s16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]});
 }
 
-// The weights' planes left in s, one at a time (and few registers) for the bf16 path.
-template <int HD, int M>
-__device__ __attribute__((always_inline)) inline void weigh_values_odd(
-    const uint16_t *lds, f32x4 (&s)[Mode<M>::columns][Mode<M>::tiles], State<HD, M> &st, uint32_t n, uint32_t g) {
-    constexpr int QT = Mode<M>::columns, NT = Mode<M>::tiles;
-#pragma unroll 1
-    for (int plane = 0; plane < 3; ++plane) {
-#pragma unroll
-        for (int h = 0; h < int(kTiles) / 2; ++h) {
-            bf16x8 p[QT];
-#pragma unroll
-            for (int qi = 0; qi < QT; ++qi) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int i = (M == kHalf ? 0 : 2 * h) + j / 4;
-                    const __bf16 x = __bf16(s[qi][i][j % 4]);
-                    p[qi][j] = M != kHalf || int(n / 8) == h ? x : __bf16(0.0f);
-                }
-            }
-#pragma unroll
-            for (int mt = 0; mt < HD / 16; ++mt) {
-                const bf16x8 a = value_fragment<HD, bf16x8>(lds, h, mt, n, g);
-#pragma unroll
-                for (int qi = 0; qi < QT; ++qi) {
-                    st.o[qi][mt] = mf::mfma(a, p[qi], st.o[qi][mt]);
-                }
-            }
-        }
-#pragma unroll
-        for (int qi = 0; qi < QT; ++qi) {
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    s[qi][i][j] -= float(__bf16(s[qi][i][j]));
-                }
-            }
-        }
-    }
-}
-
-template <int HD, class V, int PP, int M>
+template <int HD, int PP, int M>
 __device__ __attribute__((always_inline)) inline void weigh_values(
     const uint16_t *lds, const f32x4 (&s)[Mode<M>::columns][Mode<M>::tiles], State<HD, M> &st, uint32_t n, uint32_t g) {
     constexpr int QT = Mode<M>::columns;
-    // fragments requested together, and a batch ahead where the registers are there
-    constexpr int kSteps = int(kTiles) / 2, kBatch = 4, kBuffers = PP == 2 ? 2 : 1;
+    // fragments requested together, and a batch ahead beside the three planes of f32 queries' weights
+    // (512 tokens at 2048: 69.4 against 70.4 us); beside two it is level to slower
+    constexpr int kSteps = int(kTiles) / 2, kBatch = 4, kBuffers = PP == 3 ? 2 : 1;
     constexpr int kFragments = kSteps * (HD / 16);
     const auto fragment = [&](int f) __attribute__((always_inline)) {
-        return value_fragment<HD, V>(lds, f / (HD / 16), f % (HD / 16), n, g);
+        return value_fragment<HD>(lds, f / (HD / 16), f % (HD / 16), n, g);
     };
-    V a[kBuffers][kBatch];
+    bf16x8 a[kBuffers][kBatch];
     const auto request = [&](int f0) __attribute__((always_inline)) {
 #pragma unroll
         for (int f = 0; f < kBatch; ++f) {
@@ -508,7 +453,7 @@ __device__ __attribute__((always_inline)) inline void weigh_values(
     if (kBuffers == 2) {
         request(0);
     }
-    V p[QT][PP];
+    bf16x8 p[QT][PP];
 #pragma unroll
     for (int f0 = 0; f0 < kFragments; f0 += kBatch) {
         const int h = f0 / (HD / 16);
@@ -522,12 +467,12 @@ __device__ __attribute__((always_inline)) inline void weigh_values(
                     x[j] = s[qi][kOwn * h][j];
                     x[4 + j] = s[qi][kOwn * h + 1][j];
                 }
-                split<V, PP>(x, p[qi]);
+                split(x, p[qi]);
                 if (M == kHalf) {  // the lane's tiles are K step 0 in columns 0..7, step 1 in 8..15
 #pragma unroll
                     for (int k = 0; k < PP; ++k) {
                         const mf::u32x4 w = __builtin_bit_cast(mf::u32x4, p[qi][k]);
-                        p[qi][k] = __builtin_bit_cast(V, int(n / 8) == h ? w : mf::u32x4{0u, 0u, 0u, 0u});
+                        p[qi][k] = __builtin_bit_cast(bf16x8, int(n / 8) == h ? w : mf::u32x4{0u, 0u, 0u, 0u});
                     }
                 }
             }
@@ -560,11 +505,11 @@ __device__ inline void store4(__bf16 *p, const f32x4 &v) {
     *reinterpret_cast<bf16x4 *>(p) = __builtin_convertvector(v, bf16x4);
 }
 
-// Planes of a type: of the queries (bf16), of the weights (f16).
+// bf16 planes of a type: of the queries, of the weights.
 template <class T>
 constexpr int kQueryPlanes = std::is_same<T, float>::value ? 3 : 1;
 template <class T>
-constexpr int kWeightPlanes = std::is_same<T, float>::value ? 2 : 1;
+constexpr int kWeightPlanes = std::is_same<T, float>::value ? 3 : 2;
 
 // The lane's query as B operand of K step s: dims g HD/4 + 8s .., in K's order.  A value that
 // is not finite makes every score NaN.
@@ -596,7 +541,7 @@ struct RawQuery {
                 v[e] = value(s, e);
                 v[e] = __builtin_isfinite(v[e]) ? (negate ? -v[e] : v[e]) : __builtin_nanf("");
             }
-            split<bf16x8, kQueryPlanes<T>>(v, out[s]);
+            split(v, out[s]);
         }
     }
 };
@@ -649,17 +594,13 @@ struct Source {
 };
 
 // A wave's chunks from `chunk` on, every kWaves-th below `end`; kc and vc hold the first one's
-// codes.  ODD false: it returns at the first chunk with a scale byte of V outside the f16
-// path's (its number, or one past the end); ODD true: it takes every chunk to the end on the
-// bf16 path.  A loop of its own for each keeps the running state in registers.  The next
-// chunk's K is requested when this one's is multiplied, its V when this one's is in LDS, into
-// the same registers.
-template <int HD, class T, int M, int TP, bool ODD>
-__device__ __attribute__((always_inline)) inline uint32_t walk(const Cache &c, const Params &a, const Source<TP> &src,
-                                                               uint32_t chunk, uint32_t end, Codes<HD> &kc,
-                                                               Codes<HD> &vc, Places<TP> here, Places<TP> next,
-                                                               uint16_t *lds, uint32_t n, uint32_t g,
-                                                               Wave<HD, M, kQueryPlanes<T>> &w) {
+// codes.  The next chunk's K is requested when this one's is multiplied, its V when this one's is
+// in LDS, into the same registers.
+template <int HD, class T, int M, int TP>
+__device__ __attribute__((always_inline)) inline void walk(const Cache &c, const Params &a, const Source<TP> &src,
+                                                           uint32_t chunk, uint32_t end, Codes<HD> &kc, Codes<HD> &vc,
+                                                           Places<TP> here, Places<TP> next, uint16_t *lds, uint32_t n,
+                                                           uint32_t g, Wave<HD, M, kQueryPlanes<T>> &w) {
     constexpr int NS = HD / 32, QP = kQueryPlanes<T>, PP = kWeightPlanes<T>, QT = Mode<M>::columns;
     constexpr int NT = Mode<M>::tiles;
     const LaneOffsets<HD> at(n, g);
@@ -671,14 +612,27 @@ __device__ __attribute__((always_inline)) inline uint32_t walk(const Cache &c, c
         if (!inside || !all_in_pool(c, here)) {
             trim_chunk<HD, TP>(c, here, chunk, src.lo, src.hi, n, kc, vc);
         }
-        if (!ODD) {
-            uint32_t far = 0;
+        uint32_t largest = vc.scale[0];
+#pragma unroll
+        for (uint32_t i = 1; i < kTiles; ++i) {
+            largest = max(largest, vc.scale[i]);
+        }
+        const bool nans = __any(largest == 255);
+        if (nans) {
+            // NaN blocks of a position, a bit each, behind the rows (its lanes are n, n + 16,
+            // n + 32, n + 48); their values are zeros from here on
 #pragma unroll
             for (uint32_t i = 0; i < kTiles; ++i) {
-                far = max(far, vc.scale[i] - kF16First);
-            }
-            if (__any(far > kF16Last - kF16First)) {
-                return chunk;
+                const bool nan = vc.scale[i] == 255;
+                const uint32_t bits = or_over_groups(nan ? 1u << (g * (HD / 4) / 32) : 0u);
+                if (g == 0) {
+                    lds[kChunk * HD + 16 * i + n] = uint16_t(bits);
+                }
+                vc.scale[i] = nan ? 127u : vc.scale[i];
+#pragma unroll
+                for (int x = 0; x < NS; ++x) {
+                    vc.w[i][x] = nan ? 0u : vc.w[i][x];
+                }
             }
         }
         const uint32_t ahead = min(chunk + kWaves, end - 1);
@@ -708,26 +662,7 @@ __device__ __attribute__((always_inline)) inline uint32_t walk(const Cache &c, c
         }
         __builtin_amdgcn_sched_barrier(0);
         load_codes<HD, TP, false>(c, src.head, src.page_bytes, here, ahead, src.lo, src.hi, at, kc);
-        if (ODD) {
-            // NaN blocks of a position, a bit each, behind the rows (its lanes are n, n + 16,
-            // n + 32, n + 48); their values are zeros here
-#pragma unroll
-            for (uint32_t i = 0; i < kTiles; ++i) {
-                const bool nan = vc.scale[i] == 255;
-                const uint32_t bits = or_over_groups(nan ? 1u << (g * (HD / 4) / 32) : 0u);
-                if (g == 0) {
-                    lds[kChunk * HD + 16 * i + n] = uint16_t(bits);
-                }
-                vc.scale[i] = nan ? 127u : vc.scale[i];
-#pragma unroll
-                for (int x = 0; x < NS; ++x) {
-                    vc.w[i][x] = nan ? 0u : vc.w[i][x];
-                }
-            }
-            stage_values<HD, bf16x8>(lds, vc, n, g);
-        } else {
-            stage_values<HD, f16x8>(lds, vc, n, g);
-        }
+        stage_values<HD>(lds, vc, n, g);
         __builtin_amdgcn_sched_barrier(0);
         load_codes<HD, TP, true>(c, src.head, src.page_bytes, here, ahead, src.lo, src.hi, at, vc);
 
@@ -746,8 +681,8 @@ __device__ __attribute__((always_inline)) inline uint32_t walk(const Cache &c, c
         softmax_step<HD, M>(s, w.st, w.mine, whole, at0, a.c);
         __builtin_amdgcn_wave_barrier();
         asm volatile("" ::: "memory");
-        if (ODD) {
-            weigh_values_odd<HD, M>(lds, s, w.st, n, g);
+        weigh_values<HD, PP, M>(lds, s, w.st, n, g);
+        if (nans) {
 #pragma unroll
             for (int i = 0; i < NT; ++i) {
 #pragma unroll
@@ -760,28 +695,14 @@ __device__ __attribute__((always_inline)) inline uint32_t walk(const Cache &c, c
                     }
                 }
             }
-        } else {
-            weigh_values<HD, f16x8, PP, M>(lds, s, w.st, n, g);
         }
         asm volatile("" ::: "memory");
         __builtin_amdgcn_wave_barrier();
         chunk += kWaves;
         if (chunk >= end) {
-            return chunk;
+            return;
         }
     }
-}
-
-// The walk on the bf16 path, which requests its first chunk again.
-template <int HD, class T, int M, int TP>
-__device__ __attribute__((always_inline)) inline void walk_odd(const Cache &c, const Params &a, const Source<TP> &src,
-                                                               uint32_t chunk, uint32_t end, uint16_t *lds, uint32_t n,
-                                                               uint32_t g, Wave<HD, M, kQueryPlanes<T>> &w) {
-    const Places<TP> here = src.places(c, chunk), next = src.places(c, min(chunk + kWaves, end - 1));
-    Codes<HD> kc, vc;
-    load_codes<HD, TP, false>(c, src.head, src.page_bytes, here, chunk, src.lo, src.hi, LaneOffsets<HD>(n, g), kc);
-    load_codes<HD, TP, true>(c, src.head, src.page_bytes, here, chunk, src.lo, src.hi, LaneOffsets<HD>(n, g), vc);
-    walk<HD, T, M, TP, true>(c, a, src, chunk, end, kc, vc, here, next, lds, n, g, w);
 }
 
 template <uint32_t W>
@@ -869,11 +790,7 @@ __device__ __attribute__((always_inline)) inline void do_block(const Cache &c, c
         raw[qi].planes(a.negate, w.qf[qi]);
     }
     if (first < end) {
-        uint16_t *const lds = sh.v[wave];
-        const uint32_t at = walk<HD, T, M, TP, false>(c, a, src, first, end, kc, vc, here, next, lds, n, g, w);
-        if (at < end) {
-            walk_odd<HD, T, M, TP>(c, a, src, at, end, lds, n, g, w);
-        }
+        walk<HD, T, M, TP>(c, a, src, first, end, kc, vc, here, next, sh.v[wave], n, g, w);
     }
 
     // the columns' states joined through LDS
@@ -1045,10 +962,10 @@ attention_split_kernel(Cache c, Batch b, Params a, Plan plan, const T *__restric
 
 // ---- many queries: the waves of a workgroup share the chunks, each with queries of its own --------
 //
-// The waves convert the chunk's tiles of 16 positions, K to bf16 and V to f16 in LDS, where all
-// of them read them; two buffers, so that the next chunk is converted while this one is used,
-// with one barrier a chunk.  A chunk with values outside the f16 path's range is found when it
-// is converted (a flag a wave, beside the buffer), and the rest of the walk takes the bf16 path.
+// The waves convert the chunk's tiles of 16 positions to bf16 in LDS, where all of them read them;
+// two buffers, so that the next chunk is converted while this one is used, with one barrier a
+// chunk.  A tile with a NaN block of V is found when it is converted (a flag a tile, beside the
+// buffer).
 
 // Its waves: 8 with one column tile of queries each, four of which convert K and four V; 4 with
 // two for f32 queries of 64, whose registers leave room for 8 waves a CU either way (4096
@@ -1068,7 +985,7 @@ template <int HD, class T>
 union TileShared {
     struct {
         uint16_t k[2][kChunk * HD], v[2][kChunk * HD];
-        uint16_t nan[kChunk], far[2][kTiles];
+        uint16_t nan[2][kChunk], nans[2][kTiles];  // NaN blocks of a position, a bit each; tiles that have any
     };
     ShareScan<Tile<HD, T>::waves> scan;
 };
@@ -1122,13 +1039,13 @@ __device__ __attribute__((always_inline)) inline uint32_t tile_page(const Cache 
 }
 
 // The lane's quarter of row n.
-template <int HD, class V>
+template <int HD>
 __device__ __attribute__((always_inline)) inline void stage_row(uint16_t *rows, uint32_t n, uint32_t g,
                                                                 const uint32_t (&w)[HD / 32], uint32_t scale) {
 #pragma unroll
     for (int s = 0; s < HD / 32; ++s) {
-        *reinterpret_cast<V *>(rows + piece_at<HD>(n, g * (HD / 32) + s)) =
-            mf::decode_as<V>(w[s], kv4::scale_of(scale));
+        *reinterpret_cast<bf16x8 *>(rows + piece_at<HD>(n, g * (HD / 32) + s)) =
+            mf::decode_step(w[s], kv4::scale_of(scale));
     }
 }
 
@@ -1227,14 +1144,25 @@ __device__ __attribute__((always_inline)) inline void do_tile(const Cache &c, co
 #pragma unroll
         for (int part = 0; part < KV; ++part) {
             if (!is_v(part)) {
-                stage_row<HD, bf16x8>(sh.k[buf] + 16 * index * HD, n, g, x[part].w, x[part].scale);
+                stage_row<HD>(sh.k[buf] + 16 * index * HD, n, g, x[part].w, x[part].scale);
                 continue;
             }
-            stage_row<HD, f16x8>(sh.v[buf] + 16 * index * HD, n, g, x[part].w, x[part].scale);
-            const bool far = __any(x[part].scale - kF16First > kF16Last - kF16First);
-            if (lane == 0) {
-                sh.far[buf][index] = far ? 1u : 0u;
+            const bool nan = x[part].scale == 255, some = __any(nan);
+            if (some) {
+                const uint32_t bits = or_over_groups(nan ? 1u << (g * (HD / 4) / 32) : 0u);
+                x[part].scale = nan ? 127u : x[part].scale;
+#pragma unroll
+                for (int s = 0; s < NS; ++s) {
+                    x[part].w[s] = nan ? 0u : x[part].w[s];
+                }
+                if (g == 0) {
+                    sh.nan[buf][16 * index + n] = uint16_t(bits);
+                }
             }
+            if (lane == 0) {
+                sh.nans[buf][index] = some ? 1u : 0u;
+            }
+            stage_row<HD>(sh.v[buf] + 16 * index * HD, n, g, x[part].w, x[part].scale);
         }
     };
     uint32_t page = tile_page<TP>(c, src, first, index);
@@ -1271,15 +1199,9 @@ __device__ __attribute__((always_inline)) inline void do_tile(const Cache &c, co
     const auto soften = [&](uint32_t chunk, f32x4 (&s)[QT][kTiles]) __attribute__((always_inline)) {
         softmax_step<HD, M>(s, st, mine, whole.has(chunk), int32_t(chunk * kChunk + 4 * g), a.c);
     };
-    uint32_t chunk = first;
 #pragma unroll 1
-    for (; chunk < end; ++chunk) {
+    for (uint32_t chunk = first; chunk < end; ++chunk) {
         const uint32_t buf = chunk % 2;
-        // every thread sees the same flags, so all of them go the same way
-        const uint32_t far = uint32_t(sh.far[buf][0] | sh.far[buf][1]) | uint32_t(sh.far[buf][2] | sh.far[buf][3]);
-        if (__builtin_amdgcn_readfirstlane(far)) {
-            break;
-        }
         f32x4 s[QT][kTiles];
         if (needed.has(chunk)) {
             scores(buf, s);
@@ -1292,55 +1214,28 @@ __device__ __attribute__((always_inline)) inline void do_tile(const Cache &c, co
         load(min(chunk + 2, end - 1), page);
         if (needed.has(chunk)) {
             soften(chunk, s);
-            weigh_values<HD, f16x8, PP, M>(sh.v[buf], s, st, n, g);
-        }
-        __syncthreads();
-    }
-    // From a chunk with values outside the f16 path's range on: V as bf16, its NaN blocks as
-    // zeros and counted apart; one buffer.
+            weigh_values<HD, PP, M>(sh.v[buf], s, st, n, g);
+            const uint32_t some = uint32_t(sh.nans[buf][0] | sh.nans[buf][1]) | uint32_t(sh.nans[buf][2] | sh.nans[buf][3]);
+            if (__builtin_amdgcn_readfirstlane(some)) {
 #pragma unroll 1
-    for (; chunk < end; ++chunk) {
-        const uint32_t here = tile_page<TP>(c, src, chunk, index);
-        load(chunk, here);
-        trim(chunk, here);
-        __syncthreads();
+                for (uint32_t i = 0; i < kTiles; ++i) {
+                    if (!sh.nans[buf][i]) {
+                        continue;  // (nothing was noted of its positions)
+                    }
 #pragma unroll
-        for (int part = 0; part < KV; ++part) {
-            if (!is_v(part)) {
-                stage_row<HD, bf16x8>(sh.k[0] + 16 * index * HD, n, g, x[part].w, x[part].scale);
-                continue;
-            }
-            const bool nan = x[part].scale == 255;
-            const uint32_t bits = or_over_groups(nan ? 1u << (g * (HD / 4) / 32) : 0u);
-            x[part].scale = nan ? 127u : x[part].scale;
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t local = 16 * i + 4 * g + j;
+                        const int32_t p = int32_t(chunk * kChunk + local);
+                        const uint32_t bits = sh.nan[buf][local];
 #pragma unroll
-            for (int i = 0; i < NS; ++i) {
-                x[part].w[i] = nan ? 0u : x[part].w[i];
-            }
-            stage_row<HD, bf16x8>(sh.v[0] + 16 * index * HD, n, g, x[part].w, x[part].scale);
-            if (g == 0) {
-                sh.nan[16 * index + n] = uint16_t(bits);
-            }
-        }
-        __syncthreads();
-        if (needed.has(chunk)) {
-            f32x4 s[QT][kTiles];
-            scores(0, s);
-            soften(chunk, s);
-            weigh_values_odd<HD, M>(sh.v[0], s, st, n, g);
-#pragma unroll
-            for (uint32_t i = 0; i < kTiles; ++i) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int32_t local = int32_t(16 * i + 4 * g) + j, p = int32_t(chunk * kChunk) + local;
-                    const uint32_t nans = sh.nan[local];
-#pragma unroll
-                    for (int qi = 0; qi < QT; ++qi) {
-                        nan_blocks[qi] |= p >= mine[qi].first && p <= mine[qi].last ? nans : 0u;
+                        for (int qi = 0; qi < QT; ++qi) {
+                            nan_blocks[qi] |= p >= mine[qi].first && p <= mine[qi].last ? bits : 0u;
+                        }
                     }
                 }
             }
         }
+        __syncthreads();
     }
 
 #pragma unroll
