@@ -977,3 +977,32 @@ def test_weights_keep_their_bits(dev, held, heads, kv_heads, hd, news, dtype):
     q, qb = to_dtype(x, dtype)
     got = run_attention(dev, held, held.up(pool.bytes), pool, table, [n], news, qb, heads, dtype, 0, 0.125, None)
     check_close(got, q, pool, table, [n], news or [1], heads, dtype, 0, 0.125, None)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,news", WAYS)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("length", [1, 2, 5, 90, 700])
+def test_the_largest_values(dev, held, heads, kv_heads, hd, news, dtype, length):
+    """V up to the largest that a block holds, or as large as positions times V stay below 2^128;
+    scores grow along the sequence, so weights do."""
+    rng = np.random.default_rng(81 + length)
+    rows, page = news[0] if news else 1, 64
+    n = max(length, rows)
+    e = min(125, int(np.floor(128 - np.log2(6 * n))))
+    pool = R.Pool(16, kv_heads, hd, page)
+    table = rng.permutation(16).astype(np.int32)[None]
+    for p in range(n):
+        k = rng.standard_normal((kv_heads, hd)) * 0.2
+        k[:, 0] = p / n
+        v = np.full((kv_heads, hd), 6.0 * 2.0 ** e)
+        v[:, 1::3] *= -1.0 / 3.0
+        v[:, 2] = 0.0
+        pool.put(table[0], p, k, v)
+    x = rng.standard_normal((rows, heads, hd)) * 0.5
+    x[:, :, 0] = np.linspace(-40, 160, heads)
+    q, qb = to_dtype(x, dtype)
+    sinks = rng.standard_normal(heads).astype(np.float32)
+    for s in (None, sinks):
+        got = run_attention(dev, held, held.up(pool.bytes), pool, table, [n], news, qb, heads, dtype, 0, 0.125, s)
+        assert np.isfinite(got).all()
+        check_close(got, q, pool, table, [n], news or [1], heads, dtype, 0, 0.125, s)

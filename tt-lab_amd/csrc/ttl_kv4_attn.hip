@@ -53,7 +53,9 @@ typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 constexpr uint32_t kChunk = 64, kTiles = kChunk / 16;
 constexpr uint32_t kWaves = 4, kThreads = kWaves * 64;
 constexpr float kLog2e = 0x1.715476p+0f, kLog2eLo = 0x1.4ae0cp-26f;  // log2 e = their sum
-constexpr float kWeightShift = 7.0f;                                // weights are held times 2^7
+// A weight is held as 2^-8 when it is the largest seen, and grows to 1 at most: what sums up in f32
+// is never more than the values' own sum, and few large values have room.
+constexpr float kWeightShift = -8.0f;
 
 // How a wave's 16 columns are used (M): kHalf for 8 queries or fewer, columns 8..15 the same
 // queries on the other half of the chunk (so that no lane weighs scores that nobody asked for:
@@ -274,7 +276,7 @@ __device__ __attribute__((always_inline)) inline bool all_in_pool(const Cache &c
 
 template <int HD, int M>
 struct State {
-    float b[Mode<M>::columns];  // offset: c x a large score - 7; weights are 2^(c s - b), 2^15 at most
+    float b[Mode<M>::columns];  // offset: c x a large score + 8; weights are 2^(c s - b), 1 at most
     float l[Mode<M>::columns];  // the lane's share of their sum
     f32x4 o[Mode<M>::columns][HD / 16];  // O^T: dims 16 mt + 4g + i of column n
 };
@@ -304,7 +306,7 @@ struct Query {
 };
 
 // Scores to weights, in place.  The offset follows the largest score lazily: it is set anew (and
-// what is there rescaled) only when a weight would pass 2^15, or before any score was seen (its
+// what is there rescaled) only when a weight would pass 1, or before any score was seen (its
 // weights would then be infinite).
 // `at`: the position of the lane's first score.
 template <int HD, int M>
@@ -339,7 +341,7 @@ __device__ __attribute__((always_inline)) inline void softmax_step(f32x4 (&s)[Mo
                 m[qi] = fmaxf(m[qi], s[qi][i][j]);
             }
         }
-        far |= fmaf(m[qi], c, -st.b[qi]) > 15.0f;
+        far |= fmaf(m[qi], c, -st.b[qi]) > 0.0f;
     }
     if (__any(far)) {
 #pragma unroll
