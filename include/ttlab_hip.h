@@ -581,7 +581,8 @@ typedef struct {
  * positions, the call's own tokens included; its rows are starts[s] .. starts[s + 1] - 1, at
  * its last positions in order.  starts NULL: one row per sequence (tokens == sequences).
  * starts[0] = 0 and starts never decreases; rows from starts[sequences] on are padding, and
- * what belongs to them is neither read nor written.  Position p of sequence s lies in page
+ * what belongs to them is neither read nor written (nor is a row from `tokens` on, where starts
+ * passes it).  Position p of sequence s lies in page
  * page_table[s][p / page_positions] (entries that hold no used position may be anything).
  * The arrays are in device memory, so one captured call serves every step; what they hold
  * is bounds-checked by the kernels: a row before position 0 (a sequence of length 0: an idle

@@ -1006,3 +1006,62 @@ def test_the_largest_values(dev, held, heads, kv_heads, hd, news, dtype, length)
         got = run_attention(dev, held, held.up(pool.bytes), pool, table, [n], news, qb, heads, dtype, 0, 0.125, s)
         assert np.isfinite(got).all()
         check_close(got, q, pool, table, [n], news or [1], heads, dtype, 0, 0.125, s)
+
+
+@pytest.mark.parametrize("news,tokens", [([3, 5], 6), ([3, 5], 2), ([90, 300], 301), ([400, 90], 120), ([700], 650)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_starts_past_the_rows(dev, held, news, tokens, dtype):
+    """Arrays that hold fewer rows than starts names: the rows that are there as in the whole call,
+    in the store, the read-back and the attention."""
+    rng = np.random.default_rng(91 + tokens)
+    heads, kv, hd, page = 8, 1, 64, 64
+    lengths = [n + 400 * s for s, n in enumerate(news)]
+    pages = sum(-(-n // page) for n in lengths)
+    pool = R.Pool(pages, kv, hd, page).randomise(rng)
+    table = R.tables(rng, lengths, page, pages)
+    total = sum(news)
+    x = rng.standard_normal((total, (heads + 2 * kv) * hd)).astype(np.float32)
+    rope, tb, lb = held.up(rope_table(max(lengths), hd, rng)), held.up(table), held.up(np.int32(lengths))
+    sb, xb = held.up(cumulative(news)), held.up(x)
+    att = T.kv4_attention(heads, dtype, 0, 0.125, None)
+    size = 2 if dtype == BF16 else 4
+    seen = []
+    for rows in (total, tokens):
+        pb = held.up(pool.bytes)
+        cache = T.kv4_cache(pb, pages, kv, hd, page)
+        batch = T.kv4_batch(len(news), rows, tb, table.shape[1], lb, sb, None, page)
+        q, out = (held.new(total * heads * hd * size, 0x5a) for _ in range(2))
+        dev.qkv_rope_store_kv4(cache, batch, heads, xb, F32, None, rope, max(lengths), q, dtype)
+        k = held.new(total * kv * hd * 4, 0x5a)
+        dev.kv4_dequantize(cache, batch, k, None)
+        stored = pb.download(np.uint8)
+        # (over the whole call's cache: the rows left out are keys of those behind them)
+        if rows == total:
+            full = cache
+        need = dev.attention_kv4_workspace_bytes(full, batch, att)
+        dev.attention_prefill_kv4(full, batch, att, q, out, held.new(need) if need else None, need)
+        seen.append((read(q, (total, heads, hd), dtype), read(k, (total, kv, hd), F32),
+                     read(out, (total, heads, hd), dtype), stored))
+    (q0, k0, o0, _), (q1, k1, o1, stored) = seen
+    assert np.array_equal(q0[:tokens], q1[:tokens]) and np.array_equal(k0[:tokens], k1[:tokens])
+    whole, row = R.Pool(pages, kv, hd, page), 0
+    whole.bytes[...] = seen[0][3].reshape(whole.bytes.shape)
+    for s, (n, m) in enumerate(zip(lengths, news)):
+        here = min(m, max(tokens - row, 0))
+        kf, vf = whole.get(table[s], np.arange(n))
+        ref, mag, smax, vsum = R.attention(q1[row:row + here], kf, vf, np.arange(n - m, n - m + here), 0, 0, 0.125, None)
+        tol = R.close_allowance(ref, mag, smax, vsum, n, hd, dtype == BF16)
+        for o in (o0, o1):
+            assert (np.abs(o[row:row + here] - ref) <= tol).all(), s
+        row += m
+    for a in (q1, k1, o1):
+        assert (a[tokens:] == a[-1, -1, -1]).all()
+    # what the rows that are there stored, and nothing else
+    after = R.Pool(pages, kv, hd, page)
+    after.bytes[...] = pool.bytes
+    at = np.concatenate([np.arange(n - m, n) for n, m in zip(lengths, news)])
+    seq = np.repeat(np.arange(len(news)), news)
+    _, kr, vr = R.rotate(x, None, rope.download(np.float32).reshape(max(lengths), hd // 2, 2), at, heads, kv, hd)
+    for i in range(tokens):
+        after.put(table[seq[i]], at[i], kr[i], vr[i])
+    assert np.array_equal(stored.reshape(after.bytes.shape), after.bytes)

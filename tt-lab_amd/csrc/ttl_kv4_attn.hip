@@ -95,7 +95,7 @@ struct Plan {
 // ---- which queries and positions a block has -----------------------------------------------
 
 struct Block {
-    uint32_t sequence, row0, rows;     // the sequence's rows
+    uint32_t sequence, row0, rows;     // the sequence's rows, those behind the arrays' end left out
     uint32_t query0;                   // the block's first query of the sequence
     int32_t position0;                 // of the sequence's first row (negative: idle rows)
     uint32_t first_chunk, chunks;      // none: no row of the block sees a position
@@ -103,9 +103,10 @@ struct Block {
     bool exists, bad;
 };
 
-__device__ inline Block block_span(const Batch &b, const Params &a, uint32_t queries, Block k) {
-    const int32_t length = kv4::entry(b.lengths, k.sequence);
-    k.position0 = length - int32_t(k.rows);
+// `all` rows: with those left out, which have the last positions.
+__device__ inline Block block_span(const Batch &b, const Params &a, uint32_t queries, Block k, uint32_t all) {
+    const int32_t length = max(kv4::entry(b.lengths, k.sequence), 0);
+    k.position0 = length - int32_t(all);
     k.bad = length > 0 && uint32_t(length) > b.max_length;
     const uint32_t last = min(k.query0 + queries, k.rows * a.group) - 1;
     const int32_t p0 = max(k.position0 + int32_t(k.query0 / a.group), 0), p1 = k.position0 + int32_t(last / a.group);
@@ -128,7 +129,7 @@ __device__ inline uint32_t units_of(const Plan &plan, const Block &k) {
 // running sum of their numbers is needed (at most one index per sequence stays unused).
 __device__ inline Block block_of(const Batch &b, const Params &a, uint32_t queries, uint32_t index) {
     Block k{};
-    uint32_t within;
+    uint32_t within, all = 1;
     if (!b.starts) {
         const uint32_t per = (a.group + queries - 1) / queries;
         k.sequence = index / per;
@@ -148,8 +149,9 @@ __device__ inline Block block_of(const Batch &b, const Params &a, uint32_t queri
         }
         k.sequence = lo;
         k.row0 = min(uint32_t(max(kv4::entry(b.starts, lo), 0)), b.tokens);
-        const uint32_t end = min(uint32_t(max(kv4::entry(b.starts, lo + 1), 0)), b.tokens);
-        k.rows = end > k.row0 ? end - k.row0 : 0;
+        const uint32_t end = uint32_t(max(kv4::entry(b.starts, lo + 1), 0));
+        all = end > k.row0 ? end - k.row0 : 0;
+        k.rows = min(all, b.tokens - k.row0);
         const uint64_t base = uint64_t(k.row0) * a.group / queries + lo;
         if (index < base) {
             return k;
@@ -161,7 +163,7 @@ __device__ inline Block block_of(const Batch &b, const Params &a, uint32_t queri
     }
     k.exists = true;
     k.query0 = within * queries;
-    return block_span(b, a, queries, k);
+    return block_span(b, a, queries, k, all);
 }
 
 // ---- the cache's codes as MFMA operands ------------------------------------------------------
