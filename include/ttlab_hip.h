@@ -634,7 +634,7 @@ int ttl_qkv_rope_store_kv4(ttl_ctx *ctx, const ttl_kv4_cache *cache, const ttl_k
 int ttl_kv4_dequantize(ttl_ctx *ctx, const ttl_kv4_cache *cache, const ttl_kv4_batch *batch, float *k_dev,
                        float *v_dev);
 
-/* Device memory that a call of the attention below needs (0: none). */
+/* Device memory that a call of the attention below needs (0: none, or a call that is refused). */
 size_t ttl_attention_kv4_workspace_bytes(const ttl_kv4_cache *cache, const ttl_kv4_batch *batch,
                                          const ttl_kv4_attention *attention);
 /* out = softmax(scale q k, sink) v of one token per sequence (batch->starts NULL) at its last

@@ -167,3 +167,35 @@ def test_calls_past_a_launch_are_refused():
     assert store(c, b) == SHAPE and b"too many" in LIB.ttl_last_error()
     assert LIB.ttl_kv4_dequantize(CTX, C.byref(c), C.byref(b), P, P) == SHAPE
     assert attend(c, b, attention(heads=64 * 8), prefill=True) == SHAPE
+
+
+class Calls:
+    """Stands for the library: keeps what the binding hands on."""
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.last = (name, [a._obj for a in args if hasattr(a, "_obj")])
+            return 0
+        return call
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
+def test_the_default_bound_is_the_page_table(page):
+    """Without a max_length the calls take what the table holds in the cache's own pages, whatever
+    kv4_batch was told of them; one that is given is kept."""
+    dev = object.__new__(T.Device)
+    dev.lib, dev.ctx = Calls(), None
+    c, a = T.kv4_cache(P, 40, 8, 64, page), T.kv4_attention(64)
+    made = [T.kv4_batch(3, 3, P, 7, P), T.kv4_batch(3, 3, P, 7, P, None, 100), T.kv4_batch(3, 3, P, 1 << 28, P),
+            T.kv4_batch(3, 3, P, 7, P)]
+    made[3].max_length = 90
+    for b, bound in zip(made, (7 * page, 100, 1 << 30, 90)):
+        for call in (lambda: dev.qkv_rope_store_kv4(c, b, 64, P, 0, P, P, 9, P, 0), lambda: dev.kv4_dequantize(c, b, P, P),
+                     lambda: dev.attention_kv4_workspace_bytes(c, b, a), lambda: dev.attention_decode_kv4(c, b, a, P, P),
+                     lambda: dev.attention_prefill_kv4(c, b, a, P, P)):
+            call()
+            _, args = dev.lib.last
+            held = args[1]
+            assert args[0] is c and held.max_length == bound
+            assert (held.sequences, held.tokens, held.table_stride, held.page_table, held.lengths, held.starts) == (
+                3, 3, b.table_stride, P, P, None)

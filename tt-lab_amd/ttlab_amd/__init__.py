@@ -112,11 +112,27 @@ def kv4_pool_bytes(pages, kv_heads=8, head_dim=64, page_positions=64):
 def kv4_batch(sequences, tokens, page_table, table_stride, lengths, starts=None, max_length=None, page_positions=64):
     """The sequences of a call: device arrays of page_table int32 [sequences][table_stride],
     lengths int32 [sequences] and starts int32 [sequences + 1] (None: one token each).
-    max_length (at least every length): by default what the page table can hold."""
-    if max_length is None:
-        max_length = table_stride * page_positions
-    return Kv4BatchDesc(sequences, tokens, table_stride, max_length, _address(page_table), _address(lengths),
-                        _address(starts))
+    max_length (at least every length): by default what the page table can hold, in pages of the
+    cache that a call of Device is given (page_positions where the descriptor is passed on directly).
+    The attention's division goes by it, so a bound near the lengths makes short ones faster."""
+    whole = _kv4_capacity(table_stride, page_positions)
+    batch = Kv4BatchDesc(sequences, tokens, table_stride, whole if max_length is None else max_length,
+                         _address(page_table), _address(lengths), _address(starts))
+    batch.default_length = whole if max_length is None else None
+    return batch
+
+
+def _kv4_capacity(table_stride, page_positions):
+    """The positions of a page table, 2^30 at most."""
+    return min(table_stride * page_positions, 1 << 30)
+
+
+def _kv4_batch_of(cache, batch):
+    """`batch` as the calls over `cache` take it, by reference."""
+    if getattr(batch, "default_length", None) == batch.max_length:  # (not one set since)
+        batch = Kv4BatchDesc.from_buffer_copy(batch)
+        batch.max_length = _kv4_capacity(batch.table_stride, cache.page_positions)
+    return C.byref(batch)
 
 
 def kv4_attention(heads, dtype=TTL_DTYPE_F32, window=0, scale=0.125, sinks=None):
@@ -865,29 +881,31 @@ class Device:
     def qkv_rope_store_kv4(self, cache, batch, heads, qkv, x_dtype, bias, rope, rope_positions, q, q_dtype,
                            tiled=False):
         """Bias, rotation and store of the batch's new tokens; q receives the queries."""
-        _check(self.lib.ttl_qkv_rope_store_kv4(self.ctx, C.byref(cache), C.byref(batch), heads, _address(qkv), x_dtype,
-                                               TTL_QKV_TILED if tiled else TTL_QKV_PLAIN, _address(bias),
-                                               _address(rope), rope_positions, _address(q), q_dtype),
+        _check(self.lib.ttl_qkv_rope_store_kv4(self.ctx, C.byref(cache), _kv4_batch_of(cache, batch), heads,
+                                               _address(qkv), x_dtype, TTL_QKV_TILED if tiled else TTL_QKV_PLAIN,
+                                               _address(bias), _address(rope), rope_positions, _address(q), q_dtype),
                "ttl_qkv_rope_store_kv4")
 
     def kv4_dequantize(self, cache, batch, k, v):
-        _check(self.lib.ttl_kv4_dequantize(self.ctx, C.byref(cache), C.byref(batch), _address(k), _address(v)),
-               "ttl_kv4_dequantize")
+        _check(self.lib.ttl_kv4_dequantize(self.ctx, C.byref(cache), _kv4_batch_of(cache, batch), _address(k),
+                                           _address(v)), "ttl_kv4_dequantize")
 
     def attention_kv4_workspace_bytes(self, cache, batch, attention):
-        return self.lib.ttl_attention_kv4_workspace_bytes(C.byref(cache), C.byref(batch), C.byref(attention))
+        """0: the call needs none, or will be refused."""
+        return self.lib.ttl_attention_kv4_workspace_bytes(C.byref(cache), _kv4_batch_of(cache, batch),
+                                                          C.byref(attention))
 
     def attention_decode_kv4(self, cache, batch, attention, q, out, workspace=None, workspace_bytes=0):
         """One token per sequence; workspace: device memory of attention_kv4_workspace_bytes()."""
-        _check(self.lib.ttl_attention_decode_kv4(self.ctx, C.byref(cache), C.byref(batch), C.byref(attention),
-                                                 _address(q), _address(out), _address(workspace), workspace_bytes),
-               "ttl_attention_decode_kv4")
+        _check(self.lib.ttl_attention_decode_kv4(self.ctx, C.byref(cache), _kv4_batch_of(cache, batch),
+                                                 C.byref(attention), _address(q), _address(out), _address(workspace),
+                                                 workspace_bytes), "ttl_attention_decode_kv4")
 
     def attention_prefill_kv4(self, cache, batch, attention, q, out, workspace=None, workspace_bytes=0):
         """Runs of tokens (the batch has starts)."""
-        _check(self.lib.ttl_attention_prefill_kv4(self.ctx, C.byref(cache), C.byref(batch), C.byref(attention),
-                                                  _address(q), _address(out), _address(workspace), workspace_bytes),
-               "ttl_attention_prefill_kv4")
+        _check(self.lib.ttl_attention_prefill_kv4(self.ctx, C.byref(cache), _kv4_batch_of(cache, batch),
+                                                  C.byref(attention), _address(q), _address(out), _address(workspace),
+                                                  workspace_bytes), "ttl_attention_prefill_kv4")
 
     def embedding_q8_0(self, table, vocab, token, out):
         _check(self.lib.ttl_embedding_q8_0(self.ctx, table.ptr, vocab, token.ptr, out.ptr), "ttl_embedding_q8_0")
