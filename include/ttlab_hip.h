@@ -646,7 +646,7 @@ size_t ttl_attention_kv4_workspace_bytes(const ttl_kv4_cache *cache, const ttl_k
  * weights go into the product with V as bf16 planes, three for an f32 output (2^-24 of a weight),
  * two for a bf16 one (2^-16); weights below 2^-118 of the largest seen so far may count as zero.
  * Weights are 1 at most where they sum up: an output overflows only where the visible positions
- * times their largest |v| pass 2^128.
+ * times their largest |v| pass 2^128.  Scores of 2^29 and more in magnitude may give NaN.
  * Results depend on nothing but the call: the same one gives the same bits.
  * workspace_dev is caller-owned, 256-byte aligned, of the size above; calls sharing one must
  * not overlap. */

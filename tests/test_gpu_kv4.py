@@ -924,6 +924,15 @@ WAYS = [(8, 1, 64, None), (8, 1, 64, [2]), (8, 1, 64, [4]), (8, 1, 64, [70]), (8
         (8, 1, 128, [2]), (8, 1, 128, [4]), (8, 1, 128, [70])]
 
 
+def put_all(pool, table_row, k, v):
+    """k, v f64 [positions][kv_heads][hd] from position 0 on."""
+    at = np.arange(len(k))
+    page, slot = np.asarray(table_row)[at // pool.page], at % pool.page
+    for x, c, b in ((k, pool.kc, pool.ks), (v, pool.vc, pool.vs)):
+        code, byte = R.quantise(x)
+        c[page, :, slot], b[page, :, slot] = R.pack(code), byte
+
+
 def check_close(got, q, pool, table, lengths, news, heads, dtype, window, scale, sinks):
     row = 0
     for s, (n, m) in enumerate(zip(lengths, news)):
@@ -968,10 +977,9 @@ def test_weights_keep_their_bits(dev, held, heads, kv_heads, hd, news, dtype):
     n = max(rows, 2)
     pool = R.Pool(5, kv_heads, hd, page)
     table = np.arange(5, dtype=np.int32)[None]
-    for p in range(n):
-        k = np.zeros((kv_heads, hd))
-        k[:, 0] = (p + 1) % 2
-        pool.put(table[0], p, k, np.full((kv_heads, hd), 1.0 - 2.0 * (p % 2)))
+    k, v = np.zeros((n, kv_heads, hd)), np.ones((n, kv_heads, hd))
+    k[::2, :, 0], v[1::2] = 1.0, -1.0
+    put_all(pool, table[0], k, v)
     x = np.zeros((rows, heads, hd))
     x[:, :, 0] = 8.0 * np.linspace(0.001, 0.011, rows * heads).reshape(rows, heads)
     q, qb = to_dtype(x, dtype)
@@ -991,13 +999,12 @@ def test_the_largest_values(dev, held, heads, kv_heads, hd, news, dtype, length)
     e = min(125, int(np.floor(128 - np.log2(6 * n))))
     pool = R.Pool(16, kv_heads, hd, page)
     table = rng.permutation(16).astype(np.int32)[None]
-    for p in range(n):
-        k = rng.standard_normal((kv_heads, hd)) * 0.2
-        k[:, 0] = p / n
-        v = np.full((kv_heads, hd), 6.0 * 2.0 ** e)
-        v[:, 1::3] *= -1.0 / 3.0
-        v[:, 2] = 0.0
-        pool.put(table[0], p, k, v)
+    k = rng.standard_normal((n, kv_heads, hd)) * 0.2
+    k[:, :, 0] = np.arange(n)[:, None] / n
+    v = np.full((n, kv_heads, hd), 6.0 * 2.0 ** e)
+    v[:, :, 1::3] *= -1.0 / 3.0
+    v[:, :, 2] = 0.0
+    put_all(pool, table[0], k, v)
     x = rng.standard_normal((rows, heads, hd)) * 0.5
     x[:, :, 0] = np.linspace(-40, 160, heads)
     q, qb = to_dtype(x, dtype)
@@ -1065,3 +1072,83 @@ def test_starts_past_the_rows(dev, held, news, tokens, dtype):
     for i in range(tokens):
         after.put(table[seq[i]], at[i], kr[i], vr[i])
     assert np.array_equal(stored.reshape(after.bytes.shape), after.bytes)
+
+
+@pytest.mark.parametrize("news", [None, [3, 1, 90, 5], [80, 70, 90, 75]])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_short_sequences_need_no_workspace(dev, held, news, dtype):
+    rng = np.random.default_rng(95)
+    heads, kv, lengths = 16, 2, [90, 200, 95, 130]
+    pool = R.Pool(12, kv, 64, 64).randomise(rng)
+    table = R.tables(rng, lengths, 64, 12)
+    each = news or [1] * 4
+    q, qb = to_dtype(rng.standard_normal((sum(each), heads, 64)), dtype)
+    cache = T.kv4_cache(held.up(pool.bytes), 12, kv, 64, 64)
+    batch = T.kv4_batch(4, sum(each), held.up(table), table.shape[1], held.up(np.int32(lengths)),
+                        held.up(cumulative(news)) if news else None, 200)
+    att = T.kv4_attention(heads, dtype, 0, 0.125, None)
+    assert dev.attention_kv4_workspace_bytes(cache, batch, att) == 0
+    out = held.new(sum(each) * heads * 64 * 4)
+    (dev.attention_prefill_kv4 if news else dev.attention_decode_kv4)(cache, batch, att, held.up(qb), out)
+    check_close(read(out, q.shape, dtype), q, pool, table, lengths, each, heads, dtype, 0, 0.125, None)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,page", [(256, 256, 64, 16), (512, 256, 128, 32)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("news", [None, [2, 3], [70, 66]])
+def test_most_kv_heads(dev, held, heads, kv_heads, hd, page, dtype, news):
+    rng = np.random.default_rng(96)
+    lengths = [300, 70]
+    pages = sum(-(-n // page) for n in lengths)
+    pool = R.Pool(pages, kv_heads, hd, page).randomise(rng)
+    table = R.tables(rng, lengths, page, pages)
+    each = news or [1, 1]
+    q, qb = to_dtype(rng.standard_normal((sum(each), heads, hd)), dtype)
+    got = run_attention(dev, held, held.up(pool.bytes), pool, table, lengths, news, qb, heads, dtype, 0, 0.125, None)
+    check_close(got, q, pool, table, lengths, each, heads, dtype, 0, 0.125, None)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,news", WAYS)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** 12, 2.0 ** 24, 2.0 ** 27])
+def test_huge_scores(dev, held, heads, kv_heads, hd, news, dtype, size):
+    """Exact scores of up to 2^29 in magnitude, the largest of them shared by three positions."""
+    n, page = 900, 64
+    pool = R.Pool(15, kv_heads, hd, page)
+    table = np.arange(15, dtype=np.int32)[None]
+    rng = np.random.default_rng(97)
+    rows = news[0] if news else 1
+    k0 = rng.choice([-3.0, -2.0, -1.0, -0.5, 0.0, 0.5, 1.0, 2.0, 3.0], n)
+    k0[[5, 300, n - rows]] = 4.0
+    k = np.zeros((n, kv_heads, hd))
+    k[:, :, 0] = k0[:, None]
+    put_all(pool, table[0], k, rng.standard_normal((n, kv_heads, hd)))
+    x = np.zeros((rows, heads, hd))
+    x[:, :, 0] = 8.0 * size * np.linspace(0.5, 1.0, heads)[None] * (1.0 + 0.25 * (np.arange(rows) % 2))[:, None] * 0.75
+    q, qb = to_dtype(x, dtype)
+    got = run_attention(dev, held, held.up(pool.bytes), pool, table, [n], news, qb, heads, dtype, 0, 0.125, None)
+    ref, mag, smax, vsum = R.attention(q, *pool.get(table[0], np.arange(n)), np.arange(n - rows, n), 0, 0, 0.125, None)
+    # (the scores are exact; their differences in units of log 2 take two roundings, 2^-23 of them, and
+    # a difference of more than 200 is a weight of zero)
+    tol = R.close_allowance(ref, mag, np.full_like(smax, min(100.0, 8.0 * size)), vsum, n, hd, dtype == BF16)
+    assert (np.abs(got - ref) <= tol).all()
+
+
+@pytest.mark.parametrize("prefill", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_very_many_sequences(dev, held, prefill, dtype):
+    """More blocks than a call divides (2^16), over shared pages: rows of one length are alike."""
+    rng = np.random.default_rng(98)
+    count, heads, page = 70001, 8, 16
+    pool = R.Pool(80, 1, 64, page).randomise(rng)
+    one = rng.permutation(80)[:70].astype(np.int32)
+    known = np.array([1, 2, 15, 16, 17, 64, 65, 300, 1100, 0])
+    lengths = known[rng.integers(0, len(known), count)]
+    table = np.tile(one[None], (count, 1))
+    q1, qb1 = to_dtype(rng.standard_normal((1, heads, 64)), dtype)
+    got = run_attention(dev, held, held.up(pool.bytes), pool, table, lengths, np.ones(count, np.int64) if prefill else None,
+                        np.ascontiguousarray(np.broadcast_to(qb1, (count, heads, 64))), heads, dtype, 0, 0.125, None)
+    for n in known:
+        rows = got[lengths == n]
+        assert len(rows) and (rows == rows[0]).all(), n
+        check_attention(rows[:1], q1, pool, table[:1], [n], [1], heads, dtype, 0, 0.125, None)

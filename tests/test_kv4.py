@@ -199,3 +199,20 @@ def test_the_default_bound_is_the_page_table(page):
             assert args[0] is c and held.max_length == bound
             assert (held.sequences, held.tokens, held.table_stride, held.page_table, held.lengths, held.starts) == (
                 3, 3, b.table_stride, P, P, None)
+
+
+def test_a_missing_workspace_is_refused():
+    """Calls that are certain to need one (a long sequence, divided) and ones that need none."""
+    c, a = cache(pages=4096), attention()
+    for b, prefill in ((batch(sequences=1, tokens=1, table_stride=2048, max_length=131072), False),
+                       (batch(sequences=1, tokens=4, table_stride=2048, max_length=131072, starts=P), True),
+                       (batch(sequences=1, tokens=300, table_stride=2048, max_length=131072, starts=P), True)):
+        need = LIB.ttl_attention_kv4_workspace_bytes(C.byref(c), C.byref(b), C.byref(a))
+        assert need > 0
+        assert attend(c, b, a, size=need - 1, prefill=prefill) == INVALID
+        assert str(need).encode() in LIB.ttl_last_error()
+        assert attend(c, b, a, size=0, prefill=prefill) == INVALID
+        assert attend(c, b, a, ws=None, size=need, prefill=prefill) == INVALID
+        assert attend(c, b, a, ws=P + 128, size=need, prefill=prefill) == INVALID
+    for b in (batch(max_length=200), batch(tokens=600, starts=P, max_length=200)):
+        assert LIB.ttl_attention_kv4_workspace_bytes(C.byref(c), C.byref(b), C.byref(a)) == 0
