@@ -23,14 +23,14 @@
 // Maxima, sums and outputs are f32.  A NaN block of V would reach rows that do not see it (a weight
 // of zero times NaN), so its values are zeros in LDS and the queries that see it are noted apart.
 //
-// What bounds them (a large copy moves 5.1 TB/s here, a large f16 product 1.18 PFLOP/s).  One
-// token a sequence: the codes are read once; 128 sequences at 4096 (289 MB, f32 queries) take 73..76
-// us with their join, 3.8 to 4.0 TB/s, 64 ragged ones up to 8192 (151 MB, bf16) 49 us, 3.1 TB/s: the vector
-// instructions of conversion and softmax, a third of the cycles, against loads that 2 or 3
-// waves a SIMD keep in flight.  Prompts: the vector instructions, half of the cycles (an exponential a
-// score costs as much as three multiply-adds, a conversion as one and a half), next to the
-// products' quarter: 4096 tokens of 64 bf16 heads of 64 take 312 us, 440 TFLOP/s (251 with the weights
-// as one f16 plane, which lost those 2^-32 and less of the largest).
+// What bounds them (a large copy moves 5.1 TB/s here, a large bf16 product 1.23 PFLOP/s).  One
+// token a sequence: the codes are read once; 128 sequences at 4096 (289 MB, f32 queries) take 77
+// us with their join, 3.8 TB/s, 64 ragged ones up to 8192 (151 MB, bf16) 49 us, 3.1 TB/s: the vector
+// instructions of conversion and softmax, 29% (bf16) and 42% (f32) of the cycles, against loads
+// that 2 or 3 waves a SIMD keep in flight.  Prompts: the vector instructions, 57% of the cycles (an
+// exponential a score costs as much as three multiply-adds, its split into two planes as two and a
+// half), next to the products' 26%: 4096 tokens of 64 bf16 heads of 64 take 313 us, 440 TFLOP/s
+// (251 with the weights as one f16 plane, which lost those 2^-32 and less of the largest).
 #include "ttl_kv4.hpp"
 #include "ttl_mfma.hpp"
 
@@ -59,7 +59,7 @@ constexpr float kWeightShift = -8.0f;
 
 // How a wave's 16 columns are used (M): kHalf for 8 queries or fewer, columns 8..15 the same
 // queries on the other half of the chunk (so that no lane weighs scores that nobody asked for:
-// 128 f32 sequences at 4096 in 72.9 instead of 74.7 us, level in bf16);
+// 128 f32 sequences at 4096 in 80 instead of 85 us, level in bf16);
 // kOne and kTwo for 16 queries, and 32 in two column tiles.
 constexpr int kHalf = 0, kOne = 1, kTwo = 2;
 template <int M>
@@ -715,9 +715,9 @@ struct ShareScan {
     uint32_t block, first;  // the share's first block, and that block's first unit
 };
 
-// Workgroups of a CU (waves of a SIMD).  More would fit on 128 registers with M kHalf, and were
-// slower: 4 instead of 3 for bf16 queries 51.7 against 49.2 us (64 ragged sequences up to
-// 8192), 3 instead of 2 for f32 78.1 against 72.6 us (128 at 4096).
+// Workgroups of a CU (waves of a SIMD).  One more would fit with M kHalf, and was slower: 4 instead
+// of 3 for bf16 queries 52.8 against 50.9 us (64 ragged sequences up to 8192), 3 instead of 2 for
+// f32 83 against 80 us (128 at 4096; 16 bytes of scratch).
 template <int HD, class T, int M>
 constexpr int kResident = M == kTwo ? (HD == 64 ? 2 : 1) : HD == 128 || std::is_same<T, float>::value ? 2 : 3;
 
@@ -973,8 +973,9 @@ attention_split_kernel(Cache c, Batch b, Params a, Plan plan, const T *__restric
 
 // Its waves: 8 with one column tile of queries each, four of which convert K and four V; 4 with
 // two for f32 queries of 64, whose registers leave room for 8 waves a CU either way (4096
-// tokens of 64 heads: 394 against 453 us; heads of 128, 2048 tokens of 20: 8 waves 124 against
-// 151 us in f32, 98 against 99 us in bf16).
+// tokens of 64 heads: 439 against 497 us, though 512 at 2048 69 against 61).  With heads of 128 two
+// column tiles spill (2048 tokens of 20 heads: 8 waves 94 against 202 us in f32, 71 against 122 in
+// bf16).
 template <int HD, class T>
 struct Tile {
     static constexpr bool wide = HD == 128 || !std::is_same<T, float>::value;
@@ -1219,7 +1220,8 @@ __device__ __attribute__((always_inline)) inline void do_tile(const Cache &c, co
         if (needed.has(chunk)) {
             soften(chunk, s);
             weigh_values<HD, PP, M>(sh.v[buf], s, st, n, g);
-            const uint32_t some = uint32_t(sh.nans[buf][0] | sh.nans[buf][1]) | uint32_t(sh.nans[buf][2] | sh.nans[buf][3]);
+            const uint32_t some = uint32_t(sh.nans[buf][0] | sh.nans[buf][1]) |
+                                  uint32_t(sh.nans[buf][2] | sh.nans[buf][3]);
             if (__builtin_amdgcn_readfirstlane(some)) {
 #pragma unroll 1
                 for (uint32_t i = 0; i < kTiles; ++i) {
@@ -1289,8 +1291,10 @@ attention_tile_kernel(Cache c, Batch b, Params a, Plan plan, const T *__restrict
 
 // W waves per row and head, P parts at a time each (HD / 4 lanes a part): 4 waves where few
 // rows may have many parts; one where rows are few; else only the lanes of one part (P = 1),
-// which takes fewer waves for what is mostly waiting (512 tokens of 64 heads at 2048: 61 against
-// 69 us with the attention, 4 tokens of 8 sequences at 16384: 35 against 33).
+// which takes fewer waves for what is mostly waiting.  In us with the attention, for W, P = 4 and
+// all, 1 and all, 1 and 1: 64 rows of 96 parts (one token at 131072) 26.8, 28.1, 26.8; 64 rows of 9
+// parts 10.9, 11.1, 12.3; 2048 rows (4 tokens of 8 sequences at 16384) 39, 37.8, 40; 4096 rows (64
+// ragged sequences) 54.3, 50.6, 50.8; 32768 rows (512 tokens at 2048) 107, 79, 71.
 template <int HD, class T, int W, int P>
 __global__ __launch_bounds__(kThreads) void attention_join_kernel(Cache c, Batch b, Params a, Plan plan,
                                                                   T *__restrict__ out) {
@@ -1409,10 +1413,10 @@ uint32_t resident_groups(uint32_t head_dim, int dtype) {
 // The cut of a checked call, by the queries that a sequence has on average: few share a
 // workgroup's waves, from kTileFrom on each wave has its own.  Heads of 64 over long contexts
 // fill a wave with less: from kTileFromLong on where a query sees more than kLongChunks (64
-// sequences of 128 queries, bf16: at 2048 the split kernel takes 97 against 116 us, with a window
-// of 128 43 against 33; of 192 queries at 1024 98 against 79, 8 of 256 at 4096 47 against 48, 64
-// of 256 with the window 76 against 43; heads of 128, 8 sequences of 200 queries at 4096: 52
-// against 43).
+// sequences of 128 queries, bf16: at 2048 the split kernel takes 108 against 146 us, with a window
+// of 128 43 against 36; of 192 queries at 1024 103 against 87, 8 of 256 at 4096 49 against 53, 64
+// of 256 with the window 78 against 45; heads of 128, 8 sequences of 200 queries at 4096: 55
+// against 48).  What a query sees goes by max_length, the bound that the call states.
 struct Cut {
     bool tile;
     int mode;
@@ -1464,11 +1468,12 @@ Cut cut_of(const ttl_kv4_cache *cache, const ttl_kv4_batch *batch, const ttl_kv4
     }
     const uint32_t chunks = longest / kChunk + (attention->window ? 2 : 1);  // any alignment
     const uint64_t units = (chunks + p.unit - 1) / p.unit;
-    // A workgroup takes a block whole where blocks are enough (1024 tokens at 2048: 61 against 87
-    // us), or short enough for half as many (4 x 128 tokens at 1024: 35 against 47 us; but 512 at
-    // 8192: 198 against 137), or so short that the join costs more than a workgroup's walk (a
-    // prompt of 300: 13 against 26 us; two of 100 at 1400, f32: 46 against 38), or so many that
-    // finding a share would take long, the units pass 31 bits or the join a grid.
+    // A workgroup takes a block whole where blocks are enough (1024 tokens at 2048: 75 against 83
+    // us), or short enough for half as many (4 x 128 tokens at 1024: 41 against 43 us; but 512 at
+    // 8192: 238 against 144), or so short that the join costs more than a workgroup's walk (a
+    // prompt of 300: 14 against 22 us; two of 100 at 1400, f32: 51 against 40), or so many that
+    // finding a share would take long, the units pass 31 bits or the join a grid.  Blocks are as long
+    // as max_length lets them be: under a bound of 131072 a prompt of 300 is divided.
     const uint64_t all = uint64_t(p.blocks) * cache->kv_heads;
     const bool whole = all >= slots || (2 * all >= slots && units <= kLongChunks) || units <= kShortChunks;
     p.single = units == 1 || (cut.tile && whole) || p.blocks > 1u << 16 || p.blocks * units > 1u << 31 ||
