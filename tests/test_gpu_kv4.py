@@ -1152,3 +1152,60 @@ def test_very_many_sequences(dev, held, prefill, dtype):
         rows = got[lengths == n]
         assert len(rows) and (rows == rows[0]).all(), n
         check_attention(rows[:1], q1, pool, table[:1], [n], [1], heads, dtype, 0, 0.125, None)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,page,news", [(16, 2, 64, 16, None), (16, 2, 64, 64, [3, 2]),
+                                                         (16, 2, 64, 16, [90, 70]),
+                                                         (10, 2, 128, 16, None), (10, 2, 128, 64, [3, 2]),
+                                                         (10, 2, 128, 16, [90, 70])])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_the_least_alignment(dev, held, heads, kv_heads, hd, page, news, dtype):
+    """Every array at the least alignment that the header names (16 bytes; 4 for index arrays and
+    sinks), and what lies next to q and out left as it was."""
+    rng = np.random.default_rng(99)
+    lengths = [130, 300]
+    pages = sum(-(-n // page) for n in lengths)
+    pool = R.Pool(pages, kv_heads, hd, page).randomise(rng)
+    table = R.tables(rng, lengths, page, pages)
+    each = news or [1, 1]
+    rows, size = sum(each), 2 if dtype == BF16 else 4
+
+    def at(a, offset):
+        a = np.ascontiguousarray(a)
+        b = held.new(a.nbytes + 64, 0x5a)
+        raw = np.full(a.nbytes + 64, 0x5a, np.uint8)
+        raw[offset:offset + a.nbytes] = a.view(np.uint8).reshape(-1)
+        b.upload(raw)
+        return b, b.ptr + offset
+
+    width = (heads + 2 * kv_heads) * hd
+    x, bias = rng.standard_normal((rows, width)).astype(np.float32), rng.standard_normal(width).astype(np.float32)
+    rope = rope_table(300, hd, rng)
+    sinks = rng.standard_normal(heads).astype(np.float32)
+    pb, pp = at(pool.bytes, 16)
+    qb, qp = at(np.full(rows * heads * hd * size, 0x5a, np.uint8), 16)
+    ob, op = at(np.full(rows * heads * hd * size, 0x5a, np.uint8), 16)
+    cache = T.kv4_cache(pp, pages, kv_heads, hd, page)
+    batch = T.kv4_batch(2, rows, at(table, 4)[1], table.shape[1], at(np.int32(lengths), 4)[1],
+                        at(cumulative(news), 4)[1] if news else None)
+    dev.qkv_rope_store_kv4(cache, batch, heads, at(x, 16)[1], F32, at(bias, 16)[1], at(rope, 16)[1], 300, qp, dtype)
+    pos = np.concatenate([np.arange(n - m, n) for n, m in zip(lengths, each)])
+    qr, kr, vr = R.rotate(x, bias, rope, pos, heads, kv_heads, hd)
+    for i, s in enumerate(np.repeat([0, 1], each)):
+        pool.put(table[s], pos[i], kr[i], vr[i])
+    raw = pb.download(np.uint8)
+    assert np.array_equal(raw[16:16 + pool.bytes.nbytes], pool.bytes.reshape(-1)) and (raw[:16] == 0x5a).all()
+    assert (raw[16 + pool.bytes.nbytes:] == 0x5a).all()
+    att = T.kv4_attention(heads, dtype, 0, 0.125, at(sinks, 4)[1])
+    need = dev.attention_kv4_workspace_bytes(cache, batch, att)
+    ws = held.new(need) if need else None
+    (dev.attention_prefill_kv4 if news else dev.attention_decode_kv4)(cache, batch, att, qp, op, ws, need)
+    got = []
+    for b in (qb, ob):
+        raw = b.download(np.uint8)
+        assert (raw[:16] == 0x5a).all() and (raw[16 + rows * heads * hd * size:] == 0x5a).all()
+        data = raw[16:16 + rows * heads * hd * size]
+        got.append((R.from_bf16(data.view(np.uint16)) if dtype == BF16 else data.view(np.float32))
+                   .reshape(rows, heads, hd).astype(np.float64))
+    assert (np.abs(got[0] - qr) <= (2.0 ** -8 if dtype == BF16 else 2.0 ** -24) * np.abs(qr) + 2.0 ** -45).all()
+    check_close(got[1], got[0], pool, table, lengths, each, heads, dtype, 0, 0.125, sinks)
