@@ -1209,3 +1209,19 @@ def test_the_least_alignment(dev, held, heads, kv_heads, hd, page, news, dtype):
                    .reshape(rows, heads, hd).astype(np.float64))
     assert (np.abs(got[0] - qr) <= (2.0 ** -8 if dtype == BF16 else 2.0 ** -24) * np.abs(qr) + 2.0 ** -45).all()
     check_close(got[1], got[0], pool, table, lengths, each, heads, dtype, 0, 0.125, sinks)
+
+
+@pytest.mark.parametrize("heads,kv_heads,hd,news", WAYS)
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("e", [-104, -112, -120, -126])
+def test_the_smallest_values(dev, held, heads, kv_heads, hd, news, dtype, e):
+    """V in blocks of the smallest scales: what f32 holds of the output, down to its subnormals."""
+    rng = np.random.default_rng(101)
+    rows, page, n = news[0] if news else 1, 64, 333
+    pool = R.Pool(16, kv_heads, hd, page)
+    table = rng.permutation(16).astype(np.int32)[None]
+    put_all(pool, table[0], rng.standard_normal((n, kv_heads, hd)),
+            rng.choice([-6.0, -3.0, -1.0, 0.5, 1.5, 2.0, 4.0], (n, kv_heads, hd)) * 2.0 ** e)
+    q, qb = to_dtype(rng.standard_normal((rows, heads, hd)), dtype)
+    got = run_attention(dev, held, held.up(pool.bytes), pool, table, [n], news, qb, heads, dtype, 0, 0.125, None)
+    check_close(got, q, pool, table, [n], news or [1], heads, dtype, 0, 0.125, None)
